@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libafb.so")
 PROBE_PATH = os.path.join(_HERE, "libafb_probe.so")      # bench.py's gather-ceiling probe (include/afb_probe.h)
 
 OK, EINVAL, ECUDA, ESTATE = 0, -1, -2, -3
+T_F32, T_F16, T_BF16 = 0, 1, 2
 MODE_F32, MODE_DEV16 = 0, 1
 FIELDS = {"rows": 0, "carried": 1, "keep_next": 2, "keep_prev": 3, "prev_row": 4, "u_pos": 5, "u_src": 6,
           "edges": 7, "post": 8, "pre": 9, "crow": 10, "t_order": 11, "t_crow": 12, "t_col": 13,
@@ -60,6 +61,14 @@ SIGNATURES = {
                                  _i64, _p, _sz, _p, _p]),
     "afb_gemm_workspace": (_sz, [_i64, _i64, _i64]),
     "afb_gemm_f32": (_int, [_i64, _i64, _i64, _f, _p, _i64, _int, _p, _i64, _int, _p, _int, _f, _p, _i64, _p, _sz, _p, _p]),
+    "afb_quantize_rows": (_int, [_i64, _i64, _int, _p, _i64, _int, _p, _p, _f, _f, _p, _i64, _p, _p]),
+    "afb_int8_matmul": (_int, [_i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _int, _i64, _p, _p]),
+    "afb_int8_linear_workspace": (_sz, [_i64, _i64]),
+    "afb_int8_linear": (_int, [_i64, _i64, _i64, _int, _p, _i64, _int, _p, _p, _f, _f, _p, _i64, _p, _p, _p, _int, _i64, _p,
+                               _sz, _p, _p]),
+    "afb_top_logits": (_int, [_i64, _i64, _int, _p, _i64, _int, _f, _p, _p, _i64, _p, _p, _p, _p]),
+    "afb_distill_loss": (_int, [_i64, _i64, _int, _p, _i64, _int, _p, _p, _p, _f, _p, _p, _i64, _p, _f, _p, _i64, _int, _p, _p,
+                                _p, _i64, _p]),
 }
 
 # the entry points of include/afb_probe.h (libafb_probe.so)

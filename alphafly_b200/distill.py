@@ -1,0 +1,154 @@
+"""Distillation: training a network on another one's best moves (the targets' selection, the loss, the step).
+
+The reference trains on the visit distributions of its own search (chessfly/train.py:105-132).  A network can
+also learn from a slower one (more steps through the wiring, another checkpoint): ``top_logits`` keeps each
+position's k best policy logits of the teacher, some 12 k bytes instead of a dense (4168,) row, and
+``distillation_loss`` is the divergence of the student's distribution from the teacher's,
+
+    loss = T^2 sum_c p_c (log p_c - log q_c)
+
+with p = softmax(teacher / T) over the k named moves and, with ``rest``, one more outcome "any other move" of
+the mass the teacher leaves to it, and q = softmax(student / T) over all moves or the legal ones.  Both run in
+libafb (``afb_top_logits``, ``afb_distill_loss``); the loss and its gradient are one pass over the logits.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .int8 import TYPES
+
+
+class TopLogits(NamedTuple):
+    """A teacher's best moves per position: ``values`` (B, k) float32 logits, largest first, ``moves`` (B, k)
+    int64 (-inf and -1 where a position has fewer), ``log_rest`` (B,) float32: log sum exp(logit / temperature)
+    of the other moves, and the ``temperature`` it was taken at."""
+    values: torch.Tensor
+    moves: torch.Tensor
+    log_rest: torch.Tensor
+    temperature: float = 1.0
+
+
+def _check_logits(logits: torch.Tensor, temperature: float) -> torch.Tensor:
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be (B, moves), got {tuple(logits.shape)}")
+    if logits.dtype not in TYPES:
+        raise TypeError(f"logits must be float32, float16 or bfloat16, not {logits.dtype}")
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be a CUDA tensor")
+    if not temperature > 0:
+        raise ValueError("the temperature must be positive")
+    return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
+
+
+def _matrix(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device, name: str) -> torch.Tensor:
+    if tuple(t.shape) != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} {shape} on the logits' device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return t.contiguous()
+
+
+def _legal(legal, logits: torch.Tensor):
+    """(moves, valid, length) of the legal-move lists, or Nones."""
+    if legal is None:
+        return None, None, 0
+    moves, valid = legal
+    if moves.dim() != 2:
+        raise ValueError(f"legal moves must be (B, K), got {tuple(moves.shape)}")
+    shape = (logits.shape[0], moves.shape[1])
+    return (_matrix(moves, shape, torch.int64, logits.device, "legal moves"),
+            _matrix(valid, shape, torch.bool, logits.device, "legal valid"), shape[1])
+
+
+def _ptr(t: torch.Tensor | None):
+    return t.data_ptr() if t is not None else None
+
+
+@torch.no_grad()
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=None) -> TopLogits:
+    """The k (at most 256) largest of each row of ``logits`` (B, moves), equal ones by the lower move; -inf and NaN
+    are never taken.  ``legal``: (moves (B, K) int64, valid (B, K) bool), as a ``train.Batch`` holds them, restricts
+    a row to its listed moves; a row without any comes back as -inf / -1."""
+    logits = _check_logits(logits, temperature)
+    if not 1 <= k <= 256:
+        raise ValueError("k must be between 1 and 256")
+    b, n = logits.shape
+    dev = logits.device
+    moves, valid, listed = _legal(legal, logits)
+    out = TopLogits(torch.empty(b, k, dtype=torch.float32, device=dev), torch.empty(b, k, dtype=torch.int64, device=dev),
+                    torch.empty(b, dtype=torch.float32, device=dev), float(temperature))
+    with torch.cuda.device(dev):
+        _lib.call("afb_top_logits", b, n, TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), k, float(temperature),
+                  _ptr(moves), _ptr(valid), listed, out.values.data_ptr(), out.moves.data_ptr(), out.log_rest.data_ptr(),
+                  torch.cuda.current_stream(dev).cuda_stream)
+    return out
+
+
+class _Distillation(torch.autograd.Function):
+    """The forward writes the gradient for an upstream gradient of 1 in the same pass over the logits.  The backward
+    recomputes the rows whose upstream gradient, read on the device, is anything else (it rounds to the logits' type
+    once, after the scaling); a second backward writes a gradient of its own."""
+
+    @staticmethod
+    def forward(ctx, logits, values, moves, log_rest, temperature, legal_moves, legal_valid, weight, reduction, differentiable):
+        b, n = logits.shape
+        dev = logits.device
+        scale = 1.0 / b if reduction == "mean" and b else 1.0
+        rows = torch.empty(b, dtype=torch.float32, device=dev)
+        total = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
+        grad = torch.empty(b, n, dtype=logits.dtype, device=dev) if differentiable else None
+        ctx.args = (temperature, scale)
+        ctx.save_for_backward(logits, values, moves, log_rest, legal_moves, legal_valid, weight)
+        ctx.grad = grad
+        _Distillation.launch(ctx.args, logits, values, moves, log_rest, legal_moves, legal_valid, weight, None, 0, False, rows, total, grad)
+        return rows if total is None else total
+
+    @staticmethod
+    def launch(args, logits, values, moves, log_rest, legal_moves, legal_valid, weight, upstream, step, skip_ones, rows, total, grad):
+        temperature, scale = args
+        b, n = logits.shape
+        dev = logits.device
+        with torch.cuda.device(dev):
+            _lib.call("afb_distill_loss", b, n, TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), values.shape[1],
+                      values.data_ptr(), moves.data_ptr(), _ptr(log_rest), temperature, _ptr(legal_moves), _ptr(legal_valid),
+                      legal_moves.shape[1] if legal_moves is not None else 0, _ptr(weight), scale, _ptr(upstream), step,
+                      int(skip_ones), _ptr(rows), _ptr(total), _ptr(grad), n, torch.cuda.current_stream(dev).cuda_stream)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        grad, ctx.grad = ctx.grad, None
+        fresh = grad is None
+        logits = ctx.saved_tensors[0]
+        if fresh:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        g = g.float()
+        step = 0 if g.dim() == 0 else g.stride(0)
+        _Distillation.launch(ctx.args, *ctx.saved_tensors, g, step, not fresh, None, None, grad)
+        return (grad,) + (None,) * 9
+
+
+def distillation_loss(logits: torch.Tensor, top: TopLogits, legal=None, rest: bool = False, weight: torch.Tensor | None = None,
+                      reduction: str = "mean") -> torch.Tensor:
+    """The divergence of the student's ``logits`` (B, moves) from the teacher's ``top`` (module docstring), with a
+    gradient by ``logits``: float32, the mean over the B positions, their sum, or (B,) with ``reduction`` "none".
+    ``legal``: the lists that restrict the student's softmax (as for ``top_logits``); a named move outside them is
+    left out.  ``rest``: the moves the teacher does not name count as one outcome.  ``weight`` (B,) float32 scales
+    the positions' losses.  A position without a named move contributes zero."""
+    logits = _check_logits(logits, top.temperature)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"unknown reduction {reduction!r}")
+    b, dev = logits.shape[0], logits.device
+    k = top.values.shape[1] if top.values.dim() == 2 else 0
+    if not 1 <= k <= 256:
+        raise ValueError("top must hold between 1 and 256 moves a position")
+    values = _matrix(top.values, (b, k), torch.float32, dev, "top.values")
+    moves = _matrix(top.moves, (b, k), torch.int64, dev, "top.moves")
+    log_rest = _matrix(top.log_rest, (b,), torch.float32, dev, "top.log_rest") if rest else None
+    legal_moves, legal_valid, _ = _legal(legal, logits)
+    if weight is not None:
+        weight = _matrix(weight.detach(), (b,), torch.float32, dev, "weight")
+    return _Distillation.apply(logits, values, moves, log_rest, float(top.temperature), legal_moves, legal_valid, weight, reduction,
+                               torch.is_grad_enabled() and logits.requires_grad)

@@ -238,6 +238,67 @@ AFB_API int afb_gemm_f32(int64_t p, int64_t q, int64_t k, float alpha, const flo
                          const float *y, int64_t ld_y, int y_trans, const float *bias, int bias_dim, float beta, float *r,
                          int64_t ld_r, void *workspace, size_t workspace_bytes, int *status, void *stream);
 
+/* ---- element types of the entry points below ------------------------------------------------------- */
+#define AFB_T_F32 0
+#define AFB_T_F16 1
+#define AFB_T_BF16 2
+
+/* ---- products in 8-bit integers ---------------------------------------------------------------------
+ * No counterpart in the reference (its heads are float32 layers, chessfly/model.py:103-105).  One scale per
+ * row of x (position) and per row of w (channel):
+ *     s_i = fl(max_k |x_ik| / 127)     q_ik = rint(fl(x_ik / s_i))     y_ij = (sum_k q_ik w_jk) s_i t_j + b_j
+ * with fl the float32 rounding and rint to the nearest even.  The sum is exact (int32); k <= 131071.  A row of
+ * zeros has s = 0, q = 0.  A row that holds an infinity or a NaN has s = NaN, q = 0: its results are NaN.
+ *
+ * afb_quantize_rows: x element (i, k) at x[i * ld_x + k] (x_trans = 0) or x[k * ld_x + i] (x_trans = 1), of
+ *   x_type.  With mean and var (k floats, else both NULL) x is first normalised like RunningNorm in eval mode:
+ *   clamp((x - mean) / sqrt(var + eps), -clip, clip).  q: int8, 16-byte aligned, row stride ld_q a multiple of
+ *   16; the bytes past k of a row are left as they are or set to 0.  scale: (rows).
+ * afb_int8_matmul: q (rows x k) and w (n x k) int8 as afb_quantize_rows lays them out, with their scales;
+ *   bias (n) float32 or NULL.  y[i * ld_y + j] of y_type, rounded once.  status: optional device int, OR-ed
+ *   with a non-zero code if one of the kernel's bounded waits gave up (never expected).
+ * afb_int8_linear: both, x quantised into the workspace (afb_int8_linear_workspace bytes; one call at a time
+ *   per workspace).  All asynchronous on `stream`. */
+AFB_API int afb_quantize_rows(int64_t rows, int64_t k, int x_type, const void *x, int64_t ld_x, int x_trans,
+                              const float *mean, const float *var, float eps, float clip, int8_t *q, int64_t ld_q,
+                              float *scale, void *stream);
+AFB_API int afb_int8_matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale,
+                            const int8_t *w, int64_t ld_w, const float *w_scale, const float *bias, void *y, int y_type,
+                            int64_t ld_y, int *status, void *stream);
+AFB_API size_t afb_int8_linear_workspace(int64_t rows, int64_t k);
+AFB_API int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, const void *x, int64_t ld_x, int x_trans,
+                            const float *mean, const float *var, float eps, float clip, const int8_t *w, int64_t ld_w,
+                            const float *w_scale, const float *bias, void *y, int y_type, int64_t ld_y, void *workspace,
+                            size_t workspace_bytes, int *status, void *stream);
+
+/* ---- distillation from a teacher's best moves ---------------------------------------------------------
+ * No counterpart in the reference, which trains on visit distributions (chessfly/train.py:105-132).
+ * logits: (rows, n_moves) of `type`, row stride ld, n_moves <= 1048576.  legal, valid: the moves that take
+ * part, (rows, n_listed) int64 and 0 / 1 bytes, n_listed <= 4096; both NULL: all moves.  A listed move that is
+ * not valid, out of range or named before in its row is ignored.  1 <= k <= 256, temperature T > 0.
+ *
+ * afb_top_logits: each row's k largest logits, largest first, equal ones by the lower move, into values and
+ *   moves (rows, k); NaN and -inf are never taken; places that no move fills hold -inf and -1.  log_rest
+ *   (rows): log sum exp(logit / T) of the row's other moves, -inf if there are none.
+ * afb_distill_loss: row_loss[i] = weight[i] T^2 sum_c p_c (log p_c - log q_c), with p the softmax of
+ *   values / T over the row's named moves and, where log_rest is given, one more outcome (any other move) of
+ *   logit log_rest[i]; q = softmax(logits / T) over the row's moves.  Named moves that do not take part, hold
+ *   -inf or are named before in the row are left out; a row with none left, or whose own logits are all -inf,
+ *   has loss and gradient 0.
+ *   weight (rows) or NULL (1).  loss (1 float): scale * sum of row_loss.  grad (type, row stride ld_grad):
+ *   scale * upstream[i * upstream_step] * the gradient of row_loss[i] by the row's logits, rounded once
+ *   (upstream NULL: 1).  With skip_ones the rows whose upstream gradient is 1 are left untouched, for a
+ *   gradient that an earlier call wrote.  row_loss, loss, grad may each be NULL (loss needs row_loss).
+ * Both asynchronous on `stream`; the same inputs give the same bits. */
+AFB_API int afb_top_logits(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k,
+                           float temperature, const int64_t *legal, const uint8_t *valid, int64_t n_listed,
+                           float *values, int64_t *moves, float *log_rest, void *stream);
+AFB_API int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k,
+                             const float *values, const int64_t *moves, const float *log_rest, float temperature,
+                             const int64_t *legal, const uint8_t *valid, int64_t n_listed, const float *weight, float scale,
+                             const float *upstream, int64_t upstream_step, int skip_ones, float *row_loss, float *loss,
+                             void *grad, int64_t ld_grad, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
