@@ -38,7 +38,16 @@ using tc::bar_init;
 using tc::fail;
 using tc::kBK;
 using tc::kMmaK;
+using tc::arrive_remote;
+using tc::cluster_count;
+using tc::cluster_id;
+using tc::cluster_rank;
+using tc::cluster_sync;
+using tc::commit_pair;
+using tc::map_to;
 using tc::smem_desc;
+using tc::tma_load_pair;
+using tc::wait_bar;
 
 constexpr int kHalf = 128;                       // W rows and x rows (positions) per CTA of the pair
 constexpr int kTileRows = 2 * kHalf;             // neurons per pair tile (MMA M)
@@ -55,61 +64,11 @@ constexpr int kSmemBytes = kStages * kStageBytes + kStagingBytes + 1024 /* barri
 constexpr uint32_t kAccCols = kTileCols;         // one accumulator: 256 float32 columns
 constexpr uint32_t kTmemCols = 2 * kAccCols;
 constexpr uint32_t kIdesc = tc::idesc_f16(kTileRows, kTileCols);
-constexpr uint32_t kWaitLimit = 1u << 22;
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_id() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%clusterid.x;\n" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_count() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%nclusterid.x;\n" : "=r"(r));
-    return r;
-}
-// The shared::cluster address of the variable at `addr` (this CTA's shared window) in CTA `rank`.
-__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
-}
-
-// Bounded wait that also gives up as soon as another thread has reported a failure.
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const int *status) {
-    for (uint32_t it = 0; it < kWaitLimit; ++it) {
-        uint32_t ok;
-        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-        if (ok) return true;
-        if ((it & 1023u) == 1023u && status && *reinterpret_cast<const volatile int *>(status) != 0) return false;
-    }
-    return false;
-}
-
-// A 2-D TMA load into this CTA's shared memory whose bytes count on an mbarrier of either CTA of the pair.
-__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar_cluster) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_cluster) : "memory");
-}
 __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t accumulate) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
                  " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(kIdesc), "r"(accumulate) : "memory");
-}
-// Arrive on an mbarrier (shared::cluster address, either CTA) once every two-SM MMA issued so far is done.
-__device__ __forceinline__ void commit_pair(uint32_t bar_cluster) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar_cluster) : "memory");
-}
-__device__ __forceinline__ void arrive_remote(uint32_t bar_cluster) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar_cluster) : "memory");
 }
 __device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y, uint32_t src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n"
@@ -318,15 +277,25 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     return encode;
 }
 
-void encode_operand(CUtensorMap *map, const void *base, int64_t rows, int64_t k_dim, int64_t ld, uint32_t box_rows) {
+// Both operand types fill a 128-byte swizzle row with one box row: 64 float16 or 128 8-bit integers.
+static void encode_rows(CUtensorMap *map, CUtensorMapDataType type, int size, const void *base, int64_t rows, int64_t k_dim,
+                        int64_t ld, uint32_t box_rows) {
     const cuuint64_t dim[2] = {(cuuint64_t)k_dim, (cuuint64_t)rows};
-    const cuuint64_t stride[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {(cuuint32_t)kBK, box_rows};
+    const cuuint64_t stride[1] = {(cuuint64_t)ld * size};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), box_rows};
     const cuuint32_t estride[2] = {1, 1};
-    const CUresult r = tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dim, stride, box,
+    const CUresult r = tensor_map_encoder()(map, type, 2, const_cast<void *>(base), dim, stride, box,
                                             estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     AFB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code " + std::to_string((int)r));
+}
+
+void encode_operand(CUtensorMap *map, const void *base, int64_t rows, int64_t k_dim, int64_t ld, uint32_t box_rows) {
+    encode_rows(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, rows, k_dim, ld, box_rows);
+}
+
+void encode_operand_s8(CUtensorMap *map, const void *base, int64_t rows, int64_t k_dim, int64_t ld, uint32_t box_rows) {
+    encode_rows(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, rows, k_dim, ld, box_rows);
 }
 
 }  // namespace tc

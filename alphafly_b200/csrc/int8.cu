@@ -12,6 +12,7 @@
 //   second finds its data in cache.
 // dot_kernel: one warp per channel and up to kRows rows, the rows' 8-bit values in shared memory, __dp4a.
 #include "dtypes.cuh"
+#include "tc.cuh"
 
 namespace afb {
 namespace {
@@ -134,6 +135,215 @@ __global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(int64_t rows, int64
     }
 }
 
+// ---- the tensor-core product --------------------------------------------------------------------------------
+
+constexpr int kHalf = 128;                       // channels per CTA of a pair
+constexpr int kBK8 = 128;                        // k per stage: one 128-byte swizzle row
+constexpr int kMmaK8 = 32;
+constexpr int kEpiWarps = 4;
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;    // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kRingBytes = 196608;               // 192 KB of stages, whatever the tile
+
+// A tile: 2 kHalf channels (MMA M) x kRows rows of y (MMA N).
+template <int kRows>
+struct Tile {
+    static constexpr int a_bytes = kHalf * kBK8, b_bytes = kRows / 2 * kBK8, stage_bytes = a_bytes + b_bytes;
+    static constexpr int stages = kRingBytes / stage_bytes;
+    static constexpr int smem = stages * stage_bytes + 1024 /* barriers */ + 1024 /* alignment */;
+    static constexpr uint32_t tmem_cols = 2 * kRows;
+    static constexpr uint32_t idesc = tc::idesc_s8(2 * kHalf, kRows);
+};
+
+__device__ __forceinline__ void mma_pair_s8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+template <typename O, int kRows>
+__global__ void __launch_bounds__(kPairThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, int rows, int n, int k_dim,
+                const float *__restrict__ q_scale, const float *__restrict__ w_scale, const float *__restrict__ bias,
+                O *__restrict__ y, int64_t ld_y, int *__restrict__ status) {
+    using S = Tile<kRows>;
+    extern __shared__ unsigned char smem_raw[];
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
+    const uint32_t ring = (raw + 1023u) & ~1023u;                        // stage s: w half, then q half
+    const uint32_t bars = ring + S::stages * S::stage_bytes;
+    auto full = [&](int s) { return bars + 8u * s; };
+    auto empty = [&](int s) { return bars + 8u * (S::stages + s); };
+    auto tfull = [&](int b) { return bars + 8u * (2 * S::stages + b); };
+    auto tempty = [&](int b) { return bars + 8u * (2 * S::stages + 2 + b); };
+    const uint32_t tmem_slot = bars + 8u * (2 * S::stages + 4);
+    unsigned char *const slot_ptr = smem_raw + (tmem_slot - raw);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const int n_kb = (k_dim + kBK8 - 1) / kBK8;
+    const int m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf);
+    const int total = m_tiles * ((rows + kRows - 1) / kRows);
+    const int first = (int)tc::cluster_id(), step = (int)tc::cluster_count();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::stages; ++s) {
+            tc::bar_init(full(s), 1);
+            tc::bar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::bar_init(tfull(b), 1);
+            tc::bar_init(tempty(b), 2 * kEpiWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
+        asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&map_q)) : "memory");
+    }
+    if (warp == 0) {                                                     // warp 0 of both CTAs allocates
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(S::tmem_cols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    tc::cluster_sync();                                                  // both CTAs' barriers are initialised
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(slot_ptr);
+
+    if (warp == 0 && lane == 0) {                                        // TMA producer (both CTAs)
+        int it = 0;
+        bool ok = true;
+        for (int t = first; t < total && ok; t += step) {
+            const int m0 = (t % m_tiles) * 2 * kHalf, i0 = (t / m_tiles) * kRows;
+            for (int kb = 0; kb < n_kb; ++kb, ++it) {
+                const int s = it % S::stages, use = it / S::stages;
+                if (use > 0 && !tc::wait_bar(empty(s), (use - 1) & 1, status)) {
+                    tc::fail(status, 1);
+                    ok = false;
+                    break;
+                }
+                const uint32_t leader_full = tc::map_to(full(s), 0);
+                if (rank == 0) tc::bar_expect_tx(full(s), 2 * S::stage_bytes);
+                const uint32_t a_dst = ring + s * S::stage_bytes, b_dst = a_dst + S::a_bytes;
+                tc::tma_load_pair(a_dst, &map_w, kb * kBK8, m0 + (int)rank * kHalf, leader_full);
+                tc::tma_load_pair(b_dst, &map_q, kb * kBK8, i0 + (int)rank * (kRows / 2), leader_full);
+            }
+        }
+    } else if (warp == 1 && lane == 0 && rank == 0) {                    // MMA issuer (leader)
+        int it = 0, ti = 0;
+        bool ok = true;
+        for (int t = first; t < total && ok; t += step, ++ti) {
+            const int b = ti & 1, use_b = ti >> 1;
+            if (use_b > 0 && !tc::wait_bar(tempty(b), (use_b - 1) & 1, status)) {
+                tc::fail(status, 2);
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const uint32_t d = tmem + (uint32_t)(b * kRows);
+            for (int kb = 0; kb < n_kb; ++kb, ++it) {
+                const int s = it % S::stages, use = it / S::stages;
+                if (!tc::wait_bar(full(s), use & 1, status)) {
+                    tc::fail(status, 4);
+                    ok = false;
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+                const uint32_t a_src = ring + s * S::stage_bytes, b_src = a_src + S::a_bytes;
+                // the last k block takes only the 32-wide steps that hold data; the others would add zero fill
+                const int nj = min(kBK8 / kMmaK8, (k_dim - kb * kBK8 + kMmaK8 - 1) / kMmaK8);
+#pragma unroll
+                for (int j = 0; j < kBK8 / kMmaK8; ++j)
+                    if (j < nj)
+                        mma_pair_s8(d, tc::smem_desc(a_src + j * kMmaK8), tc::smem_desc(b_src + j * kMmaK8), S::idesc,
+                                    (kb > 0 || j > 0) ? 1u : 0u);
+                tc::commit_pair(empty(s));                               // the stage is free in both CTAs once
+                tc::commit_pair(tc::map_to(empty(s), 1));                // these MMAs have read it
+            }
+            if (!ok) break;
+            tc::commit_pair(tfull(b));                                   // the accumulator is complete
+            tc::commit_pair(tc::map_to(tfull(b), 1));
+        }
+    } else if (warp >= 2) {                                              // epilogue (both CTAs)
+        const int quarter = warp & 3;
+        const uint32_t leader_tempty[2] = {tc::map_to(tempty(0), 0), tc::map_to(tempty(1), 0)};
+        int ti = 0;
+        for (int t = first; t < total; t += step, ++ti) {
+            const int b = ti & 1, use_b = ti >> 1;
+            const int m = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf + quarter * 32 + lane, i0 = (t / m_tiles) * kRows;
+            if (!__all_sync(0xffffffffu, tc::wait_bar(tfull(b), use_b & 1, status))) {
+                if (lane == 0) tc::fail(status, 8);
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const float ws = m < n ? w_scale[m] : 0.f, bm = m < n && bias ? bias[m] : 0.f;
+            O *const out = y + (int64_t)i0 * ld_y + m;
+#pragma unroll 1
+            for (int c = 0; c < kRows / 32; ++c) {
+                if (i0 + c * 32 >= rows) break;                          // uniform over the warp
+                const float mine = i0 + c * 32 + lane < rows ? q_scale[i0 + c * 32 + lane] : 0.f;
+                uint32_t r[32];
+                tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * kRows + c * 32), r);
+                tc::tmem_wait_ld();
+                // lanes run along the channels: one row's store is one line
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                    const float qs = __shfl_sync(0xffffffffu, mine, j);
+                    if (m < n && i0 + c * 32 + j < rows)
+                        out[(int64_t)(c * 32 + j) * ld_y] = from_float<O>(fmaf((float)(int)r[j] * ws, qs, bm));
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) tc::arrive_remote(leader_tempty[b]);          // this accumulator is drained
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+    tc::cluster_sync();                                                  // both CTAs are done with TMEM and barriers
+    if (warp == 0) {
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::tmem_cols) : "memory");
+    }
+}
+
+// Pairs of CTAs that the device holds at once (one CTA per SM).
+int device_pairs() {
+    static int pairs[64] = {0};
+    int dev = 0;
+    AFB_CUDA(cudaGetDevice(&dev));
+    AFB_CHECK(dev >= 0 && dev < 64, "device index out of range");
+    if (!pairs[dev]) {
+        int sms = 0;
+        AFB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        pairs[dev] = sms / 2;
+    }
+    return pairs[dev];
+}
+
+template <typename O, int kRows>
+void launch_pairs(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w,
+                  int64_t ld_w, const float *w_scale, const float *bias, O *y, int64_t ld_y, int *status, cudaStream_t s) {
+    using S = Tile<kRows>;
+    CUtensorMap map_w, map_q;
+    tc::encode_operand_s8(&map_w, w, n, k, ld_w, kHalf);
+    tc::encode_operand_s8(&map_q, q, rows, k, ld_q, kRows / 2);
+    const int64_t total = (n + 2 * kHalf - 1) / (2 * kHalf) * ((rows + kRows - 1) / kRows);
+    AFB_CHECK(total < (1LL << 31), "too many rows for one launch");
+    const int64_t pairs = std::min<int64_t>(total, device_pairs());
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
+    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.dynamicSmemBytes = S::smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O, kRows>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
+    AFB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<O, kRows>, map_w, map_q, (int)rows, (int)n, (int)k, q_scale, w_scale, bias, y,
+                                ld_y, status));
+}
+
 void check_rows16(const void *p, int64_t ld, const char *what) {
     AFB_CHECK((reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 16 == 0, std::string(what) + " rows must start on 16-byte boundaries");
 }
@@ -154,7 +364,22 @@ void quantize(int64_t rows, int64_t k, int type, const void *x, int64_t ld_x, in
 }
 
 void matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w, int64_t ld_w,
-            const float *w_scale, const float *bias, void *y, int y_type, int64_t ld_y, int *, cudaStream_t s) {
+            const float *w_scale, const float *bias, void *y, int y_type, int64_t ld_y, int *status, cudaStream_t s) {
+    if (rows > kDotRows) {
+        with_type(y_type, [&](auto t) {
+            using O = decltype(t);
+            O *out = static_cast<O *>(y);
+            // the tile that takes the fewest rounds of its size; the wide one moves the fewest bytes a product
+            const int64_t m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf), pairs = device_pairs();
+            auto cost = [&](int64_t r, int64_t unit) { return ((m_tiles * ((rows + r - 1) / r) + pairs - 1) / pairs) * unit; };
+            const int64_t c256 = cost(256, 32), c128 = cost(128, 24), c64 = cost(64, 20);
+            auto go = [&](auto tile) { launch_pairs<O, decltype(tile)::value>(rows, n, k, q, ld_q, q_scale, w, ld_w, w_scale, bias, out, ld_y, status, s); };
+            if (c256 <= c128 && c256 <= c64) go(std::integral_constant<int, 256>{});
+            else if (c128 <= c64) go(std::integral_constant<int, 128>{});
+            else go(std::integral_constant<int, 64>{});
+        });
+        return;
+    }
     const dim3 grid((unsigned)((n + kDotWarps - 1) / kDotWarps), (unsigned)((rows + kDotRows - 1) / kDotRows));
     AFB_CHECK(grid.y < 65536, "too many rows for one launch");
     with_type(y_type, [&](auto t) {

@@ -1,4 +1,4 @@
-// Shared pieces of the library's tcgen05 / TMA kernels (inmap.cu, readout.cu): mbarriers with bounded
+// Shared pieces of the library's tcgen05 / TMA kernels (inmap.cu, readout.cu, gemm.cu, int8.cu): mbarriers with bounded
 // waits, 2-D TMA loads, the shared-memory descriptor of a K-major SWIZZLE_128B float16 operand tile, the
 // kind::f16 instruction descriptor, and the tensor-map encoder.
 #pragma once
@@ -17,6 +17,12 @@ constexpr int kMmaK = 16;                       // K of one tcgen05.mma kind::f1
 // Instruction descriptor of tcgen05.mma kind::f16: D float32 (bits 4-5 = 1), A and B float16 (bits 7-9,
 // 10-12 = 0), both K-major (bits 15, 16 = 0), N >> 3 in bits 17-22, M >> 4 in bits 24-28.
 constexpr uint32_t idesc_f16(int m, int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24); }
+
+// Instruction descriptor of tcgen05.mma kind::i8: D int32 (bits 4-5 = 2), A and B signed 8-bit (bits 7-9, 10-12 = 1),
+// the rest as above.
+constexpr uint32_t idesc_s8(int m, int n) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
 
 // Shared-memory descriptor of a K-major SWIZZLE_128B operand tile whose rows are 128 bytes and whose
 // 8-row groups are 1024 bytes apart: start address >> 4 (bits 0-13), leading byte offset 16 B >> 4
@@ -63,6 +69,57 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
 }
 
+// ---- pairs of CTAs (clusters of two) and the two-SM MMA --------------------------------------------------
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_id() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%clusterid.x;\n" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_count() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%nclusterid.x;\n" : "=r"(r));
+    return r;
+}
+// The shared::cluster address of the variable at `addr` (this CTA's shared window) in CTA `rank`.
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+
+// Bounded wait that also gives up as soon as another thread has reported a failure.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const int *status) {
+    for (uint32_t it = 0; it < kWaitLimit; ++it) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+        if (ok) return true;
+        if ((it & 1023u) == 1023u && status && *reinterpret_cast<const volatile int *>(status) != 0) return false;
+    }
+    return false;
+}
+
+// A 2-D TMA load into this CTA's shared memory whose bytes count on an mbarrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar_cluster) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar_cluster) : "memory");
+}
+// Arrive on an mbarrier (shared::cluster address, either CTA) once every two-SM MMA issued so far is done.
+__device__ __forceinline__ void commit_pair(uint32_t bar_cluster) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar_cluster) : "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t bar_cluster) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar_cluster) : "memory");
+}
 // 32 consecutive float32 columns of this warp's 32 TMEM lanes (lane quarter by warp), one per register.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
@@ -81,6 +138,9 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 // A K-major float16 operand: rows x k_dim elements, row stride ld elements (a multiple of 8), boxes of
 // box_rows x 64, SWIZZLE_128B; rows and columns past the extents read as zero.
 void encode_operand(CUtensorMap *map, const void *base, int64_t rows, int64_t k_dim, int64_t ld, uint32_t box_rows);
+
+// The same of 8-bit integers: row stride ld bytes (a multiple of 16), boxes of box_rows x 128.
+void encode_operand_s8(CUtensorMap *map, const void *base, int64_t rows, int64_t k_dim, int64_t ld, uint32_t box_rows);
 
 }  // namespace tc
 }  // namespace afb
