@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(int64_t rows, int64
 constexpr int kHalf = 128;                       // channels per CTA of a pair
 constexpr int kBK8 = 128;                        // k per stage: one 128-byte swizzle row
 constexpr int kMmaK8 = 32;
-constexpr int kEpiWarps = 4;
-constexpr int kPairThreads = 64 + 32 * kEpiWarps;    // warp 0 TMA, warp 1 MMA, warps 2-5 epilogue
+constexpr int kEpiWarps = 8;                      // two for each quarter of the TMEM lanes
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;    // warp 0 TMA, warp 1 MMA, the rest epilogue
 constexpr int kRingBytes = 196608;               // 192 KB of stages, whatever the tile
 
 // A tile: 2 kHalf channels (MMA M) x kRows rows of y (MMA N).
@@ -261,37 +261,51 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             tc::commit_pair(tc::map_to(tfull(b), 1));
         }
     } else if (warp >= 2) {                                              // epilogue (both CTAs)
-        const int quarter = warp & 3;
-        const uint32_t leader_tempty[2] = {tc::map_to(tempty(0), 0), tc::map_to(tempty(1), 0)};
+        const int quarter = warp & 3, part = (warp - 2) >> 2;            // lanes, and half of the tile's rows
+        constexpr int kPart = kRows / 2;
+        const uint32_t leader_tempty0 = tc::map_to(tempty(0), 0), leader_tempty1 = tc::map_to(tempty(1), 0);
         int ti = 0;
         for (int t = first; t < total; t += step, ++ti) {
             const int b = ti & 1, use_b = ti >> 1;
-            const int m = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf + quarter * 32 + lane, i0 = (t / m_tiles) * kRows;
+            const int m = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf + quarter * 32 + lane, i0 = (t / m_tiles) * kRows + part * kPart;
+            // this tile's scales, fetched while its products run: lane l holds those of rows 32 c + l
+            const float ws = m < n ? w_scale[m] : 0.f, bm = m < n && bias ? bias[m] : 0.f;
+            float qs[kPart / 32];
+#pragma unroll
+            for (int c = 0; c < kPart / 32; ++c) qs[c] = i0 + c * 32 + lane < rows ? q_scale[i0 + c * 32 + lane] : 0.f;
             if (!__all_sync(0xffffffffu, tc::wait_bar(tfull(b), use_b & 1, status))) {
                 if (lane == 0) tc::fail(status, 8);
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const float ws = m < n ? w_scale[m] : 0.f, bm = m < n && bias ? bias[m] : 0.f;
-            O *const out = y + (int64_t)i0 * ld_y + m;
-#pragma unroll 1
-            for (int c = 0; c < kRows / 32; ++c) {
-                if (i0 + c * 32 >= rows) break;                          // uniform over the warp
-                const float mine = i0 + c * 32 + lane < rows ? q_scale[i0 + c * 32 + lane] : 0.f;
-                uint32_t r[32];
-                tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * kRows + c * 32), r);
-                tc::tmem_wait_ld();
-                // lanes run along the channels: one row's store is one line
+            O *out = y + (int64_t)i0 * ld_y + m;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float qs = __shfl_sync(0xffffffffu, mine, j);
-                    if (m < n && i0 + c * 32 + j < rows)
-                        out[(int64_t)(c * 32 + j) * ld_y] = from_float<O>(fmaf((float)(int)r[j] * ws, qs, bm));
+            for (int c = 0; c < kPart / 32; ++c) {
+                const int left = rows - i0 - c * 32;
+                if (left <= 0) break;                                    // uniform over the warp
+                uint32_t r[32];
+                tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * kRows + part * kPart + c * 32), r);
+                tc::tmem_wait_ld();
+                O v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    v[j] = from_float<O>(fmaf((float)(int)r[j] * ws, __shfl_sync(0xffffffffu, qs[c], j), bm));
+                // lanes run along the channels: one row's store is one line
+                if (m < n) {
+                    if (left >= 32) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) out[j * ld_y] = v[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (j < left) out[j * ld_y] = v[j];
+                    }
                 }
+                out += 32 * ld_y;
             }
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
-            if (lane == 0) tc::arrive_remote(leader_tempty[b]);          // this accumulator is drained
+            if (lane == 0) tc::arrive_remote_relaxed(b ? leader_tempty1 : leader_tempty0);          // this accumulator is drained
         }
     }
     __syncwarp();

@@ -117,6 +117,11 @@ __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *m
 __device__ __forceinline__ void commit_pair(uint32_t bar_cluster) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar_cluster) : "memory");
 }
+// As arrive_remote, without ordering this thread's memory accesses before the arrival: for a warp that only read TMEM (its loads
+// waited for, then tcgen05.fence::before_thread_sync).  A release would wait for the warp's global stores first.
+__device__ __forceinline__ void arrive_remote_relaxed(uint32_t bar_cluster) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar_cluster) : "memory");
+}
 __device__ __forceinline__ void arrive_remote(uint32_t bar_cluster) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(bar_cluster) : "memory");
 }
