@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t tmem_slot = bars + 8u * (2 * S::stages + 4);
     unsigned char *const slot_ptr = smem_raw + (tmem_slot - raw);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_rank();
     const int n_kb = (k_dim + kBK8 - 1) / kBK8;
     const int m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf);
@@ -226,39 +226,39 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 tc::tma_load_pair(b_dst, &map_q, kb * kBK8, i0 + (int)rank * (kRows / 2), leader_full);
             }
         }
-    } else if (warp == 1 && lane == 0 && rank == 0) {                    // MMA issuer (leader)
-        int it = 0, ti = 0;
+    } else if (warp == 1 && rank == 0) {                                 // MMA issuer (leader): the whole warp, so that
+        int it = 0, ti = 0;                                              // its state is uniform; one lane issues
         bool ok = true;
+        const bool issuer = tc::elect_one();
         for (int t = first; t < total && ok; t += step, ++ti) {
             const int b = ti & 1, use_b = ti >> 1;
-            if (use_b > 0 && !tc::wait_bar(tempty(b), (use_b - 1) & 1, status)) {
-                tc::fail(status, 2);
+            if (use_b > 0 && !__all_sync(0xffffffffu, tc::wait_bar(tempty(b), (use_b - 1) & 1, status))) {
+                if (issuer) tc::fail(status, 2);
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const uint32_t d = tmem + (uint32_t)(b * kRows);
             for (int kb = 0; kb < n_kb; ++kb, ++it) {
                 const int s = it % S::stages, use = it / S::stages;
-                if (!tc::wait_bar(full(s), use & 1, status)) {
-                    tc::fail(status, 4);
+                if (!__all_sync(0xffffffffu, tc::wait_bar(full(s), use & 1, status))) {
+                    if (issuer) tc::fail(status, 4);
                     ok = false;
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                const uint32_t a_src = ring + s * S::stage_bytes, b_src = a_src + S::a_bytes;
+                const uint32_t a_src = ring + s * S::stage_bytes;
+                const uint64_t a_desc = tc::smem_desc(a_src), b_desc = tc::smem_desc(a_src + S::a_bytes);
                 // the last k block takes only the 32-wide steps that hold data; the others would add zero fill
                 const int nj = min(kBK8 / kMmaK8, (k_dim - kb * kBK8 + kMmaK8 - 1) / kMmaK8);
+                if (issuer) {
 #pragma unroll
-                for (int j = 0; j < kBK8 / kMmaK8; ++j)
-                    if (j < nj)
-                        mma_pair_s8(d, tc::smem_desc(a_src + j * kMmaK8), tc::smem_desc(b_src + j * kMmaK8), S::idesc,
-                                    (kb > 0 || j > 0) ? 1u : 0u);
-                tc::commit_pair(empty(s));                               // the stage is free in both CTAs once
-                tc::commit_pair(tc::map_to(empty(s), 1));                // these MMAs have read it
+                    for (int j = 0; j < kBK8 / kMmaK8; ++j)              // a step of 32 bytes: 2 in the descriptor's units
+                        if (j < nj) mma_pair_s8(d, a_desc + 2 * j, b_desc + 2 * j, S::idesc, (kb > 0 || j > 0) ? 1u : 0u);
+                    tc::commit_both(empty(s));                           // the stage is free in both CTAs once these
+                    if (kb == n_kb - 1) tc::commit_both(tfull(b));       // MMAs have read it; the accumulator is complete
+                }
+                __syncwarp();
             }
-            if (!ok) break;
-            tc::commit_pair(tfull(b));                                   // the accumulator is complete
-            tc::commit_pair(tc::map_to(tfull(b), 1));
         }
     } else if (warp >= 2) {                                              // epilogue (both CTAs)
         const int quarter = warp & 3, part = (warp - 2) >> 2;            // lanes, and half of the tile's rows
