@@ -47,6 +47,7 @@ using tc::commit_pair;
 using tc::map_to;
 using tc::smem_desc;
 using tc::tma_load_pair;
+using tc::tma_store;
 using tc::wait_bar;
 
 constexpr int kHalf = 128;                       // W rows and x rows (positions) per CTA of the pair
@@ -70,11 +71,6 @@ __device__ __forceinline__ void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint6
                  " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(kIdesc), "r"(accumulate) : "memory");
 }
-__device__ __forceinline__ void tma_store(const CUtensorMap *map, int x, int y, uint32_t src) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src) : "memory");
-}
-
 __global__ void __launch_bounds__(kThreads, 1) input_map_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                 const __grid_constant__ CUtensorMap map_x,
                                                                 const __grid_constant__ CUtensorMap map_u, int n_in,

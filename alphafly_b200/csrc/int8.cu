@@ -11,6 +11,8 @@
 //   magnitudes' bits, which order like the magnitudes and put NaN on top) and one that divides and packs; the
 //   second finds its data in cache.
 // dot_kernel: one warp per channel and up to kRows rows, the rows' 8-bit values in shared memory, __dp4a.
+#include <cstring>
+
 #include "dtypes.cuh"
 #include "tc.cuh"
 
@@ -140,16 +142,18 @@ __global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(int64_t rows, int64
 constexpr int kHalf = 128;                       // channels per CTA of a pair
 constexpr int kBK8 = 128;                        // k per stage: one 128-byte swizzle row
 constexpr int kMmaK8 = 32;
-constexpr int kEpiWarps = 8;                      // two for each quarter of the TMEM lanes
-constexpr int kPairThreads = 64 + 32 * kEpiWarps;    // warp 0 TMA, warp 1 MMA, the rest epilogue
 constexpr int kRingBytes = 196608;               // 192 KB of stages, whatever the tile
+constexpr int kSlotBytes = 2048;                 // an epilogue warp stages 32 channels x 16 (float32) or 32 rows, twice
 
 // A tile: 2 kHalf channels (MMA M) x kRows rows of y (MMA N).
 template <int kRows>
 struct Tile {
     static constexpr int a_bytes = kHalf * kBK8, b_bytes = kRows / 2 * kBK8, stage_bytes = a_bytes + b_bytes;
     static constexpr int stages = kRingBytes / stage_bytes;
-    static constexpr int smem = stages * stage_bytes + 1024 /* barriers */ + 1024 /* alignment */;
+    static constexpr int parts = kRows >= 64 ? 2 : 1;                    // epilogue warps per quarter of the TMEM lanes
+    static constexpr int epi_warps = 4 * parts;
+    static constexpr int threads = 64 + 32 * epi_warps;                  // warp 0 TMA, warp 1 MMA, the rest epilogue
+    static constexpr int smem = stages * stage_bytes + epi_warps * 2 * kSlotBytes + 1024 /* barriers */ + 1024 /* alignment */;
     static constexpr uint32_t tmem_cols = 2 * kRows;
     static constexpr uint32_t idesc = tc::idesc_s8(2 * kHalf, kRows);
 };
@@ -161,15 +165,17 @@ __device__ __forceinline__ void mma_pair_s8(uint32_t d_tmem, uint64_t a_desc, ui
 }
 
 template <typename O, int kRows>
-__global__ void __launch_bounds__(kPairThreads, 1)
-    pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q, int rows, int n, int k_dim,
-                const float *__restrict__ q_scale, const float *__restrict__ w_scale, const float *__restrict__ bias,
-                O *__restrict__ y, int64_t ld_y, int *__restrict__ status) {
+__global__ void __launch_bounds__(Tile<kRows>::threads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q,
+                const __grid_constant__ CUtensorMap map_y, int rows, int n, int k_dim, const float *__restrict__ q_scale,
+                const float *__restrict__ w_scale, const float *__restrict__ bias, O *__restrict__ y, int64_t ld_y, int n_tma,
+                int *__restrict__ status) {
     using S = Tile<kRows>;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;                        // stage s: w half, then q half
-    const uint32_t bars = ring + S::stages * S::stage_bytes;
+    const uint32_t staging = ring + S::stages * S::stage_bytes;          // epilogue warp e, slot q
+    const uint32_t bars = staging + S::epi_warps * 2 * kSlotBytes;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (S::stages + s); };
     auto tfull = [&](int b) { return bars + 8u * (2 * S::stages + b); };
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             tc::bar_init(tfull(b), 1);
-            tc::bar_init(tempty(b), 2 * kEpiWarps);
+            tc::bar_init(tempty(b), 2 * S::epi_warps);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
@@ -261,10 +267,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             }
         }
     } else if (warp >= 2) {                                              // epilogue (both CTAs)
-        const int quarter = warp & 3, part = (warp - 2) >> 2;            // lanes, and half of the tile's rows
-        constexpr int kPart = kRows / 2;
+        const int quarter = warp & 3, part = (warp - 2) >> 2;            // lanes, and share of the tile's rows
+        constexpr int kPart = kRows / S::parts;
         const uint32_t leader_tempty0 = tc::map_to(tempty(0), 0), leader_tempty1 = tc::map_to(tempty(1), 0);
-        int ti = 0;
+        int ti = 0, slot = 0;
         for (int t = first; t < total; t += step, ++ti) {
             const int b = ti & 1, use_b = ti >> 1;
             const int m = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf + quarter * 32 + lane, i0 = (t / m_tiles) * kRows + part * kPart;
@@ -278,10 +284,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            O *out = y + (int64_t)i0 * ld_y + m;
 #pragma unroll
             for (int c = 0; c < kPart / 32; ++c) {
-                const int left = rows - i0 - c * 32;
+                const int i = i0 + c * 32, left = rows - i;
                 if (left <= 0) break;                                    // uniform over the warp
                 uint32_t r[32];
                 tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * kRows + part * kPart + c * 32), r);
@@ -290,23 +295,35 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
                     v[j] = from_float<O>(fmaf((float)(int)r[j] * ws, __shfl_sync(0xffffffffu, qs[c], j), bm));
-                // lanes run along the channels: one row's store is one line
-                if (m < n) {
-                    if (left >= 32) {
+                // lanes run along the channels: one row of the chunk is one line, in shared memory or of y
+                if (n_tma > 0) {
+                    constexpr int kSlotRows = kSlotBytes / (32 * (int)sizeof(O));
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) out[j * ld_y] = v[j];
-                    } else {
+                    for (int h = 0; h < 32 / kSlotRows; ++h, slot ^= 1) {
+                        O *const dst = reinterpret_cast<O *>(smem_raw + (staging - raw) + ((warp - 2) * 2 + slot) * kSlotBytes) + lane;
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");   // the slot is free
+                        __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (j < left) out[j * ld_y] = v[j];
+                        for (int j = 0; j < kSlotRows; ++j) dst[j * 32] = v[h * kSlotRows + j];
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0 && m < n_tma && h * kSlotRows < left)   // what lies past the map is clipped
+                            tc::tma_store(&map_y, m, i + h * kSlotRows, staging + (uint32_t)((warp - 2) * 2 + slot) * kSlotBytes);
+                        if (lane == 0) asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                     }
                 }
-                out += 32 * ld_y;
+                if (m >= n_tma && m < n) {
+                    O *const out = y + (int64_t)i * ld_y + m;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (j < left) out[j * ld_y] = v[j];
+                }
             }
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) tc::arrive_remote_relaxed(b ? leader_tempty1 : leader_tempty0);          // this accumulator is drained
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -315,6 +332,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::tmem_cols) : "memory");
     }
+}
+
+// y: rows x n elements of O (n whole 16-byte units: a store rounds its row up to one), row stride ld, boxes of one staging slot (32 channels).
+template <typename O>
+void encode_result(CUtensorMap *map, O *y, int64_t rows, int64_t n, int64_t ld) {
+    const cuuint64_t dim[2] = {(cuuint64_t)n, (cuuint64_t)rows};
+    const cuuint64_t stride[1] = {(cuuint64_t)ld * sizeof(O)};
+    const cuuint32_t box[2] = {32u, (cuuint32_t)(kSlotBytes / (32 * sizeof(O)))};
+    const cuuint32_t estride[2] = {1, 1};
+    const CUtensorMapDataType type = sizeof(O) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    const CUresult r = tc::tensor_map_encoder()(map, type, 2, y, dim, stride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    AFB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (result) failed with code " + std::to_string((int)r));
 }
 
 // Pairs of CTAs that the device holds at once (one CTA per SM).
@@ -335,9 +366,14 @@ template <typename O, int kRows>
 void launch_pairs(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w,
                   int64_t ld_w, const float *w_scale, const float *bias, O *y, int64_t ld_y, int *status, cudaStream_t s) {
     using S = Tile<kRows>;
-    CUtensorMap map_w, map_q;
+    CUtensorMap map_w, map_q, map_y;
     tc::encode_operand_s8(&map_w, w, n, k, ld_w, kHalf);
     tc::encode_operand_s8(&map_q, q, rows, k, ld_q, kRows / 2);
+    // the channels that TMA stores: all but the last few, or none where y's rows do not start on 16 bytes
+    const int unit = 16 / (int)sizeof(O);
+    const int n_tma = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && ld_y % unit == 0 ? (int)n / unit * unit : 0;
+    if (n_tma) encode_result(&map_y, y, rows, n_tma, ld_y);
+    else std::memset(&map_y, 0, sizeof(map_y));
     const int64_t total = (n + 2 * kHalf - 1) / (2 * kHalf) * ((rows + kRows - 1) / kRows);
     AFB_CHECK(total < (1LL << 31), "too many rows for one launch");
     const int64_t pairs = std::min<int64_t>(total, device_pairs());
@@ -348,14 +384,14 @@ void launch_pairs(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t l
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
-    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.blockDim = dim3(S::threads, 1, 1);
     cfg.dynamicSmemBytes = S::smem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O, kRows>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
-    AFB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<O, kRows>, map_w, map_q, (int)rows, (int)n, (int)k, q_scale, w_scale, bias, y,
-                                ld_y, status));
+    AFB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<O, kRows>, map_w, map_q, map_y, (int)rows, (int)n, (int)k, q_scale, w_scale,
+                                bias, y, ld_y, n_tma, status));
 }
 
 void check_rows16(const void *p, int64_t ld, const char *what) {

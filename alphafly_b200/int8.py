@@ -91,7 +91,9 @@ def _result(rows: int, n: int, k: int, w, w_scale, bias, out_dtype, device):
     if w.dim() != 2 or w.shape[1] != k:
         raise ValueError(f"inner dimensions differ: k = {k} and w {tuple(w.shape)}")
     w = _rows16(w, device, "w")
-    return w, _vector(w_scale, n, device, "w_scale"), _vector(bias, n, device, "bias"), torch.empty(rows, n, dtype=out_dtype, device=device)
+    unit = 4 if out_dtype == torch.float32 else 8                 # rows on 16 bytes: the kernel's stores are whole sectors
+    y = torch.empty(rows, -(-n // unit) * unit, dtype=out_dtype, device=device)[:, :n]
+    return w, _vector(w_scale, n, device, "w_scale"), _vector(bias, n, device, "bias"), y
 
 
 def _empty_sum(y: torch.Tensor, bias, x_scale=None) -> torch.Tensor:
@@ -103,7 +105,8 @@ def _empty_sum(y: torch.Tensor, bias, x_scale=None) -> torch.Tensor:
 @torch.no_grad()
 def int8_matmul(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
-    """(q w^T) * scale[:, None] * w_scale + bias, (rows, n) of ``out_dtype`` (rounded once).  q (rows, k) and
+    """(q w^T) * scale[:, None] * w_scale + bias, (rows, n) of ``out_dtype`` (rounded once), a view whose rows start
+    on 16-byte boundaries.  q (rows, k) and
     w (n, k) int8 as ``quantize`` returns them (other layouts are copied), k <= 131071."""
     if q.dim() != 2:
         raise ValueError(f"q must be (rows, k), got {tuple(q.shape)}")
@@ -118,7 +121,7 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: 
         return _empty_sum(y, bias)
     with torch.cuda.device(dev):
         _lib.call("afb_int8_matmul", rows, n, k, q.data_ptr(), q.stride(0), scale.data_ptr(), w.data_ptr(), w.stride(0),
-                  w_scale.data_ptr(), bias.data_ptr() if bias is not None else None, y.data_ptr(), TYPES[out_dtype], n,
+                  w_scale.data_ptr(), bias.data_ptr() if bias is not None else None, y.data_ptr(), TYPES[out_dtype], y.stride(0),
                   _device_status(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
     return y
 
@@ -128,7 +131,7 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``quantize(x, norm)`` times the quantised weight: x (rows, k) float32, float16 or bfloat16, contiguous or a
     transposed view; w (n, k) int8 and w_scale (n,) from ``quantize``; bias (n,) float32.  (rows, n) of
-    ``out_dtype``."""
+    ``out_dtype``, a view whose rows start on 16-byte boundaries."""
     _check_source(x, norm)
     rows, k = x.shape
     n, dev = w.shape[0], x.device
@@ -141,6 +144,6 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
     with torch.cuda.device(dev):
         _lib.check(lib.afb_int8_linear(rows, n, k, TYPES[x.dtype], x.data_ptr(), ld, trans, *_norm_args(norm), w.data_ptr(),
                                        w.stride(0), w_scale.data_ptr(), bias.data_ptr() if bias is not None else None,
-                                       y.data_ptr(), TYPES[out_dtype], n, ws.data_ptr(), ws.numel(),
+                                       y.data_ptr(), TYPES[out_dtype], y.stride(0), ws.data_ptr(), ws.numel(),
                                        _device_status(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
     return y
