@@ -213,23 +213,27 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(slot_ptr);
 
-    if (warp == 0 && lane == 0) {                                        // TMA producer (both CTAs)
-        int it = 0;
+    if (warp == 0) {                                                     // TMA producer (both CTAs), a converged warp
+        const bool issuer = tc::elect_one();
+        const uint32_t leader_bars = tc::map_to(bars, 0);                // `full` comes first
+        int s = 0, use = 0;
         bool ok = true;
         for (int t = first; t < total && ok; t += step) {
-            const int m0 = (t % m_tiles) * 2 * kHalf, i0 = (t / m_tiles) * kRows;
-            for (int kb = 0; kb < n_kb; ++kb, ++it) {
-                const int s = it % S::stages, use = it / S::stages;
-                if (use > 0 && !tc::wait_bar(empty(s), (use - 1) & 1, status)) {
-                    tc::fail(status, 1);
+            const int m0 = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf, i0 = (t / m_tiles) * kRows + (int)rank * (kRows / 2);
+            for (int kb = 0; kb < n_kb; ++kb) {
+                if (use > 0 && !__all_sync(0xffffffffu, tc::wait_bar(empty(s), (use - 1) & 1, status))) {
+                    if (issuer) tc::fail(status, 1);
                     ok = false;
                     break;
                 }
-                const uint32_t leader_full = tc::map_to(full(s), 0);
-                if (rank == 0) tc::bar_expect_tx(full(s), 2 * S::stage_bytes);
-                const uint32_t a_dst = ring + s * S::stage_bytes, b_dst = a_dst + S::a_bytes;
-                tc::tma_load_pair(a_dst, &map_w, kb * kBK8, m0 + (int)rank * kHalf, leader_full);
-                tc::tma_load_pair(b_dst, &map_q, kb * kBK8, i0 + (int)rank * (kRows / 2), leader_full);
+                if (issuer) {
+                    const uint32_t a_dst = ring + s * S::stage_bytes;
+                    if (rank == 0) tc::bar_expect_tx(full(s), 2 * S::stage_bytes);
+                    tc::tma_load_pair(a_dst, &map_w, kb * kBK8, m0, leader_bars + 8u * s);
+                    tc::tma_load_pair(a_dst + S::a_bytes, &map_q, kb * kBK8, i0, leader_bars + 8u * s);
+                }
+                __syncwarp();
+                if (++s == S::stages) s = 0, ++use;
             }
         }
     } else if (warp == 1 && rank == 0) {                                 // MMA issuer (leader): the whole warp, so that
