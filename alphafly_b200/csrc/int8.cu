@@ -7,10 +7,9 @@
 // kMaxK = 2^17 - 1 of them.  A row of zeros has s = 0 and q = 0; a row that holds an infinity or a NaN has
 // s = NaN and q = 0, so its results are NaN and no other row's.
 //
-// quantize_rows_kernel, quantize_columns_kernel: one pass for the largest magnitude (integer maxima of the
-//   magnitudes' bits, which order like the magnitudes and put NaN on top) and one that divides and packs; the
-//   second finds its data in cache.
-// dot_kernel: one warp per channel and up to kRows rows, the rows' 8-bit values in shared memory, __dp4a.
+// Kernels: quantize_rows_kernel and quantize_columns_kernel by the layout of x, dot_kernel for a few rows (quantisation
+// and product in one launch), pair_kernel for the rest, on the tensor cores.  The largest magnitude of a row is an
+// integer maximum of the magnitudes' bits, which order like the magnitudes and put NaN on top.
 #include <cstring>
 
 #include "dtypes.cuh"
@@ -26,11 +25,34 @@ constexpr unsigned kInfBits = 0x7f800000u;
 __device__ __forceinline__ float row_scale(unsigned amax_bits) {
     return amax_bits >= kInfBits ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(amax_bits), kTop);
 }
-// The quotient is within 127 (1 + 2^-23) unless the scale is subnormal, where it can round further up.
-__device__ __forceinline__ int quantize_one(float x, float scale) {
-    if (!(scale > 0.f)) return 0;
-    return (int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -kTop), kTop);
+// rint(fl(x / scale)) as a byte, by the division.  The quotient is within 127 (1 + 2^-23) unless the scale is subnormal,
+// where it can round further up.  0 for a scale of 0 or NaN.
+__device__ __noinline__ uint32_t quantize_by_division(float x, float scale) {
+    if (!(scale > 0.f)) return 0u;
+    return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -kTop), kTop) & 0xffu;
 }
+// Four of them with inv = fl(1 / scale).  t = x inv is off x / scale by less than 1.6e-5 (127 times two roundings), the
+// rounded quotient by 7.6e-6: unless t lies within 4e-5 of a half, both round to the same whole number, which
+// t + 1.5 2^23 holds in its low bits.  One element in 12,000 takes the division, and so do the scales whose reciprocal
+// is infinite and rows without one (inv NaN).  Rounding and conversion instructions run at a quarter of the rate.
+__device__ __forceinline__ uint32_t quantize4(float x0, float x1, float x2, float x3, float scale, float inv) {
+    constexpr float kMagic = 12582912.f;
+    const float x[4] = {x0, x1, x2, x3};
+    float f[4];
+    bool near = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float t = x[e] * inv;
+        f[e] = t + kMagic;
+        near |= !(fabsf(t - (f[e] - kMagic)) < 0.49996f);
+    }
+    if (near)
+        return quantize_by_division(x0, scale) | quantize_by_division(x1, scale) << 8 | quantize_by_division(x2, scale) << 16 |
+               quantize_by_division(x3, scale) << 24;
+    return __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
+                       __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
+}
+__device__ __forceinline__ float inverse(float scale) { return scale > 0.f ? 1.f / scale : __uint_as_float(0x7fc00000u); }
 __device__ __forceinline__ unsigned magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // RunningNorm in eval mode, as the readout applies it; without statistics the value itself.
@@ -39,102 +61,272 @@ struct Norm {
     float eps, clip;
     __device__ __forceinline__ float operator()(float x, int64_t k) const {
         if (!mean) return x;
-        return fminf(fmaxf((x - mean[k]) / sqrtf(var[k] + eps), -clip), clip);
+        const float v = (x - mean[k]) / sqrtf(var[k] + eps);
+        return v < -clip ? -clip : v > clip ? clip : v;          // NaN stays NaN
     }
 };
 
-constexpr int kRowThreads = 128;
-
-// One CTA per row of x (element (i, k) at x[i ld + k]).
+// 16 bytes of x: kPer elements.
 template <typename T>
+struct Piece {
+    static constexpr int kPer = 16 / (int)sizeof(T);
+    union {
+        uint4 raw;
+        T e[kPer];
+    };
+    __device__ __forceinline__ Piece() : raw(make_uint4(0u, 0u, 0u, 0u)) {}
+};
+
+constexpr int kRowThreads = 128;
+constexpr int kRowPieces = 8;                    // most 16-byte pieces a thread keeps
+
+// One CTA per row of x (element (i, k) at x[i ld + k]), P pieces a thread.  The row is read in 16-byte pieces wherever it
+// starts and, up to 4,080 float32 or 8,176 16-bit elements, kept in registers (longer rows are read again, from cache); the quantised
+// bytes are shifted to their place through shared memory and leave as 16-byte words, zero past k.
+template <typename T, int P>
 __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int64_t k_dim, const T *__restrict__ x, int64_t ld, Norm norm,
                                                                     int8_t *__restrict__ q, int64_t ld_q,
                                                                     float *__restrict__ scale) {
+    constexpr int kPer = Piece<T>::kPer, kSpan = kRowThreads * P * kPer;
+    constexpr int kStep = kSpan - 16;            // elements a span writes: it starts up to 7 before its first
     __shared__ unsigned amax;
+    __shared__ uint32_t bytes[kSpan / 4];
     const int64_t i = blockIdx.x;
     const T *row = x + i * ld;
+    const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     if (threadIdx.x == 0) amax = 0u;
     __syncthreads();
+    Piece<T> mine[P];
+    auto first_of = [&](int64_t base, int p) { return base + (int64_t)(p * kRowThreads + threadIdx.x) * kPer - lead; };
+    auto load = [&](int64_t base) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int64_t k = first_of(base, p);
+            mine[p] = Piece<T>();
+            if (k >= 0 && k + kPer <= k_dim) mine[p].raw = __ldg(reinterpret_cast<const uint4 *>(row + k));
+            else if (k < k_dim)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    if (k + e >= 0 && k + e < k_dim) mine[p].e[e] = row[k + e];
+        }
+    };
+    auto value = [&](int64_t base, int p, int e) {
+        const float v = to_float(mine[p].e[e]);
+        if (!norm.mean) return v;
+        const int64_t k = first_of(base, p) + e;
+        return k >= 0 && k < k_dim ? norm(v, k) : 0.f;
+    };
     unsigned m = 0u;
-    for (int64_t k = threadIdx.x; k < k_dim; k += kRowThreads) m = max(m, magnitude(norm(to_float(row[k]), k)));
+    for (int64_t base = 0; base < k_dim; base += kStep) {
+        load(base);
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) m = max(m, magnitude(value(base, p, e)));
+    }
     m = __reduce_max_sync(0xffffffffu, m);
     if ((threadIdx.x & 31) == 0) atomicMax(&amax, m);
     __syncthreads();
-    const float s = row_scale(amax);
+    const float s = row_scale(amax), inv = inverse(s);
     if (threadIdx.x == 0) scale[i] = s;
-    for (int64_t k = threadIdx.x; k < k_dim; k += kRowThreads)
-        q[i * ld_q + k] = (int8_t)quantize_one(norm(to_float(row[k]), k), s);
+    for (int64_t base = 0; base < k_dim; base += kStep) {
+        if (k_dim > kStep) load(base);
+#pragma unroll
+        for (int p = 0; p < P; ++p)                             // byte b of the span: element base - lead + b
+#pragma unroll
+            for (int w = 0; w < kPer / 4; ++w) {
+                uint32_t word = 0u;
+                if (first_of(base, p) < k_dim)
+                    word = quantize4(value(base, p, 4 * w), value(base, p, 4 * w + 1), value(base, p, 4 * w + 2), value(base, p, 4 * w + 3), s, inv);
+                bytes[(p * kRowThreads + threadIdx.x) * (kPer / 4) + w] = word;
+            }
+        __syncthreads();
+        const int n = (int)min((int64_t)kStep, k_dim - base);
+        for (int b = threadIdx.x * 16; b < n; b += kRowThreads * 16) {
+            uint32_t w[5];
+#pragma unroll
+            for (int e = 0; e < 5; ++e) w[e] = bytes[(b + lead) / 4 + e];
+            const int by = 8 * ((b + lead) & 3);
+            *reinterpret_cast<uint4 *>(q + i * ld_q + base + b) =
+                make_uint4(__funnelshift_r(w[0], w[1], by), __funnelshift_r(w[1], w[2], by), __funnelshift_r(w[2], w[3], by),
+                           __funnelshift_r(w[3], w[4], by));
+        }
+        __syncthreads();
+    }
 }
 
-constexpr int kColRows = 32;                    // rows of the result per CTA, one per lane
-constexpr int kColWarps = 16;
-constexpr int kColK = 64;                       // k per shared tile
+constexpr int kColRows = 32;                     // rows of the result per cluster, one per lane
+constexpr int kColCluster = 8;                   // CTAs of a cluster: shares of k
+constexpr int kColWarps = 8;
+constexpr int kColKeep = 40;                     // values a thread keeps
+constexpr int kColSpan = kColWarps * kColKeep;   // 320
 
-// The transposed layout: element (i, k) at x[k ld + i].  A CTA takes kColRows rows; lanes run along them.
+// The transposed layout: element (i, k) at x[k ld + i], lanes along the rows i.  A cluster of 8 CTAs shares 32 rows,
+// each CTA an eighth of k; the CTAs' largest magnitudes meet through distributed shared memory.  Up to k = 2,560 the
+// values stay in registers (beyond it they are read again, from cache); the bytes are transposed in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(32 * kColWarps) quantize_columns_kernel(int64_t rows, int64_t k_dim, const T *__restrict__ x,
-                                                                          int64_t ld, Norm norm, int8_t *__restrict__ q,
-                                                                          int64_t ld_q, float *__restrict__ scale) {
+__global__ void __cluster_dims__(kColCluster, 1, 1) __launch_bounds__(32 * kColWarps)
+    quantize_columns_kernel(int64_t rows, int64_t k_dim, const T *__restrict__ x, int64_t ld, Norm norm, int8_t *__restrict__ q,
+                            int64_t ld_q, float *__restrict__ scale) {
     __shared__ unsigned amax[kColRows];
-    __shared__ int8_t tile[kColRows][kColK + 4];
+    __shared__ __align__(16) int8_t tile[kColRows][kColSpan + 16];    // rows 21 words of 16 bytes apart
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t i0 = (int64_t)blockIdx.x * kColRows, i = i0 + lane;
+    const int64_t i0 = (int64_t)(blockIdx.x / kColCluster) * kColRows, i = i0 + lane;
+    // this CTA's share of k, in whole 16-byte words
+    const int64_t share = ((k_dim + kColCluster - 1) / kColCluster + 15) / 16 * 16;
+    const int64_t k0 = share * tc::cluster_rank(), k1 = min(k0 + share, k_dim);
     if (threadIdx.x < kColRows) amax[threadIdx.x] = 0u;
     __syncthreads();
+    float mine[kColKeep];
+    auto k_of = [&](int p) { return (p / 4 * kColWarps + warp) * 4 + p % 4; };
+    auto load = [&](int64_t base) {
+#pragma unroll
+        for (int p = 0; p < kColKeep; ++p) {
+            const int64_t k = base + k_of(p);
+            mine[p] = i < rows && k < k1 ? to_float(x[k * ld + i]) : 0.f;
+        }
+        if (norm.mean)
+#pragma unroll
+            for (int p = 0; p < kColKeep; ++p) {
+                const int64_t k = base + k_of(p);
+                if (i < rows && k < k1) mine[p] = norm(mine[p], k);
+            }
+    };
     unsigned m = 0u;
-    if (i < rows)
-        for (int64_t k = warp; k < k_dim; k += kColWarps) m = max(m, magnitude(norm(to_float(x[k * ld + i]), k)));
+    for (int64_t base = k0; base < k1; base += kColSpan) {
+        load(base);
+#pragma unroll
+        for (int p = 0; p < kColKeep; ++p) m = max(m, magnitude(mine[p]));
+    }
     atomicMax(&amax[lane], m);
+    tc::cluster_sync();
+    const uint32_t own = (uint32_t)__cvta_generic_to_shared(&amax[lane]);
+    m = 0u;
+#pragma unroll
+    for (int c = 0; c < kColCluster; ++c) {
+        unsigned v;
+        asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(tc::map_to(own, (uint32_t)c)) : "memory");
+        m = max(m, v);
+    }
+    const float s = row_scale(m), inv = inverse(s);
+    if (k0 == 0 && warp == 0 && i < rows) scale[i] = s;
+    for (int64_t base = k0; base < k1; base += kColSpan) {
+        if (share > kColSpan) load(base);
+        __syncthreads();                         // the tile's readers are done
+#pragma unroll
+        for (int p = 0; p < kColKeep; p += 4)    // a thread's four values are neighbours in k
+            *reinterpret_cast<uint32_t *>(&tile[lane][k_of(p)]) = quantize4(mine[p], mine[p + 1], mine[p + 2], mine[p + 3], s, inv);
+        __syncthreads();
+        const int words = (int)((min((int64_t)kColSpan, k1 - base) + 15) / 16);
+        for (int e = threadIdx.x; e < kColRows * words; e += 32 * kColWarps) {
+            const int r = e / words, w = e % words;
+            if (i0 + r < rows)
+                *reinterpret_cast<uint4 *>(q + (i0 + r) * ld_q + base + 16 * w) = *reinterpret_cast<const uint4 *>(&tile[r][16 * w]);
+        }
+    }
+    tc::cluster_sync();                          // no CTA ends while another may read its maxima
+}
+
+// ---- few rows ------------------------------------------------------------------------------------------------
+
+constexpr int kDotWarps = 8;
+constexpr int kDotRows = 8;                      // most rows of this path
+constexpr int kAhead = 5;                        // 16-byte words of w a lane fetches before the rows are at hand
+
+__device__ __forceinline__ int dot16(const uint4 &a, const uint4 &b, int acc) {
+    acc = __dp4a((int)a.x, (int)b.x, acc);
+    acc = __dp4a((int)a.y, (int)b.y, acc);
+    acc = __dp4a((int)a.z, (int)b.z, acc);
+    return __dp4a((int)a.w, (int)b.w, acc);
+}
+
+// y = x w^T for up to R rows in one launch: every CTA quantises the rows into shared memory (kFused; else copies them
+// from q) while its first words of w are on the way, then each warp takes one channel.  Bound by latency: w is 9.7 MB
+// at 2333 x 4171, all of it in flight at once.
+template <typename T, typename O, int R, bool kFused>
+__global__ void __launch_bounds__(32 * kDotWarps)
+    dot_kernel(int rows, int64_t n, int k_dim, const T *__restrict__ x, int64_t row_step, int64_t k_step, Norm norm,
+               const float *__restrict__ q_scale, const int8_t *__restrict__ w, int64_t ld_w, const float *__restrict__ w_scale,
+               const float *__restrict__ bias, O *__restrict__ y, int64_t ld_y) {
+    extern __shared__ uint4 held[];              // R rows of `words` 16-byte words, zero past k_dim
+    __shared__ unsigned amax[R];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, words = (k_dim + 15) / 16;
+    const int64_t j = (int64_t)blockIdx.x * kDotWarps + warp;
+    // w's last word may hold anything past k_dim: the rows hold zeros there
+    const uint4 *const wr = reinterpret_cast<const uint4 *>(w + (j < n ? j : 0) * ld_w);
+    uint4 ahead[kAhead];
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) ahead[a] = lane + 32 * a < words ? __ldg(wr + lane + 32 * a) : make_uint4(0u, 0u, 0u, 0u);
+    int8_t *const bytes = reinterpret_cast<int8_t *>(held);
+    if (kFused) {
+        if (threadIdx.x < R) amax[threadIdx.x] = 0u;
+        __syncthreads();
+        for (int r = 0; r < rows; ++r) {
+            unsigned m = 0u;
+            for (int k = threadIdx.x; k < k_dim; k += 32 * kDotWarps)
+                m = max(m, magnitude(norm(to_float(x[r * row_step + k * k_step]), k)));
+            m = __reduce_max_sync(0xffffffffu, m);
+            if (lane == 0) atomicMax(&amax[r], m);
+        }
+        __syncthreads();
+        for (int r = 0; r < rows; ++r) {
+            const float s = row_scale(amax[r]), inv = inverse(s);
+            auto value = [&](int k) { return k < k_dim ? norm(to_float(x[r * row_step + k * k_step]), k) : 0.f; };
+            for (int k = threadIdx.x * 4; k < words * 16; k += 128 * kDotWarps)
+                *reinterpret_cast<uint32_t *>(bytes + r * words * 16 + k) = quantize4(value(k), value(k + 1), value(k + 2), value(k + 3), s, inv);
+        }
+    } else {
+        for (int e = threadIdx.x; e < rows * words * 16; e += 32 * kDotWarps) {
+            const int r = e / (words * 16), k = e % (words * 16);
+            bytes[e] = k < k_dim ? (int8_t)x[r * row_step + k] : (int8_t)0;
+        }
+    }
     __syncthreads();
-    const float s = row_scale(amax[lane]);
-    if (warp == 0 && i < rows) scale[i] = s;
-    for (int64_t k0 = 0; k0 < k_dim; k0 += kColK) {
-        for (int kk = warp; kk < kColK; kk += kColWarps) {
-            const int64_t k = k0 + kk;
-            tile[lane][kk] = (i < rows && k < k_dim) ? (int8_t)quantize_one(norm(to_float(x[k * ld + i]), k), s) : (int8_t)0;
-        }
-        __syncthreads();
-        for (int e = threadIdx.x; e < kColRows * kColK; e += 32 * kColWarps) {
-            const int r = e / kColK, kk = e % kColK;
-            if (i0 + r < rows && k0 + kk < k_dim) q[(i0 + r) * ld_q + k0 + kk] = tile[r][kk];
-        }
-        __syncthreads();
+    if (j >= n) return;
+    int acc[R] = {};
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a)
+        if (lane + 32 * a < words)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (r < rows) acc[r] = dot16(held[r * words + lane + 32 * a], ahead[a], acc[r]);
+    for (int c = lane + 32 * kAhead; c < words; c += 32) {
+        const uint4 wv = __ldg(wr + c);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            if (r < rows) acc[r] = dot16(held[r * words + c], wv, acc[r]);
+    }
+    const float ws = w_scale[j], b = bias ? bias[j] : 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        if (r >= rows) break;
+        const int v = __reduce_add_sync(0xffffffffu, acc[r]);
+        const float s = kFused ? row_scale(amax[r]) : q_scale[r];
+        if (lane == r) y[r * ld_y + j] = from_float<O>(fmaf((float)v * ws, s, b));
     }
 }
 
-constexpr int kDotWarps = 8;
-constexpr int kDotRows = 8;
+// At most kDotRows rows, their bytes within the shared memory of a CTA.
+bool few_rows(int64_t rows, int64_t k) { return rows <= kDotRows && rows * ((k + 15) / 16 * 16) <= 96 * 1024; }
 
-// y rows [kDotRows blockIdx.y, ...), channels [kDotWarps blockIdx.x, ...): one warp per channel.  Rows of q and w
-// start on 16 bytes; the 16-byte words past k_dim are not read, and the last word's bytes past it are cleared.
-template <typename O>
-__global__ void __launch_bounds__(32 * kDotWarps) dot_kernel(int64_t rows, int64_t n, int k_dim, const int8_t *__restrict__ q,
-                                                             int64_t ld_q, const float *__restrict__ q_scale,
-                                                             const int8_t *__restrict__ w, int64_t ld_w,
-                                                             const float *__restrict__ w_scale, const float *__restrict__ bias,
-                                                             O *__restrict__ y, int64_t ld_y) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t j = (int64_t)blockIdx.x * kDotWarps + warp, i0 = (int64_t)blockIdx.y * kDotRows;
-    if (j >= n) return;
-    int acc[kDotRows] = {};
-    const int full = k_dim & ~3;
-    const int8_t *wr = w + j * ld_w;
-    for (int k = lane * 4; k < full; k += 128) {
-        const int wv = *reinterpret_cast<const int *>(wr + k);
-#pragma unroll
-        for (int r = 0; r < kDotRows; ++r)
-            if (i0 + r < rows) acc[r] = __dp4a(*reinterpret_cast<const int *>(q + (i0 + r) * ld_q + k), wv, acc[r]);
-    }
-    for (int k = full + lane; k < k_dim; k += 32)
-#pragma unroll
-        for (int r = 0; r < kDotRows; ++r)
-            if (i0 + r < rows) acc[r] += (int)q[(i0 + r) * ld_q + k] * (int)wr[k];
-#pragma unroll
-    for (int r = 0; r < kDotRows; ++r) {
-        const int v = __reduce_add_sync(0xffffffffu, acc[r]);
-        if (lane == 0 && i0 + r < rows)
-            y[(i0 + r) * ld_y + j] = from_float<O>(fmaf((float)v * w_scale[j], q_scale[i0 + r], bias ? bias[j] : 0.f));
-    }
+template <typename T, bool kFused>
+void launch_dot(int64_t rows, int64_t n, int64_t k, const T *x, int64_t row_step, int64_t k_step, const Norm &norm,
+                const float *q_scale, const int8_t *w, int64_t ld_w, const float *w_scale, const float *bias, void *y, int y_type,
+                int64_t ld_y, cudaStream_t s) {
+    const size_t shared = (size_t)rows * ((k + 15) / 16 * 16);
+    with_type(y_type, [&](auto t) {
+        using O = decltype(t);
+        auto go = [&](auto r) {
+            auto kernel = dot_kernel<T, O, decltype(r)::value, kFused>;
+            if (shared > 48 * 1024) AFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
+            kernel<<<(unsigned)((n + kDotWarps - 1) / kDotWarps), 32 * kDotWarps, shared, s>>>(
+                (int)rows, n, (int)k, x, row_step, k_step, norm, q_scale, w, ld_w, w_scale, bias, static_cast<O *>(y), ld_y);
+        };
+        if (rows == 1) go(std::integral_constant<int, 1>{});
+        else if (rows <= 4) go(std::integral_constant<int, 4>{});
+        else go(std::integral_constant<int, 8>{});
+    });
+    AFB_LAUNCHED();
 }
 
 // ---- the tensor-core product --------------------------------------------------------------------------------
@@ -145,18 +337,14 @@ constexpr int kMmaK8 = 32;
 constexpr int kRingBytes = 196608;               // 192 KB of stages, whatever the tile
 constexpr int kSlotBytes = 2048;                 // an epilogue warp stages 32 channels x 16 (float32) or 32 rows
 
-// A tile: 2 kHalf channels (MMA M) x kRows rows of y (MMA N).
-template <int kRows>
-struct Tile {
-    static constexpr int a_bytes = kHalf * kBK8, b_bytes = kRows / 2 * kBK8, stage_bytes = a_bytes + b_bytes;
-    static constexpr int stages = kRingBytes / stage_bytes;
-    static constexpr int parts = kRows >= 128 ? 4 : 2;                    // epilogue warps per quarter of the TMEM lanes
-    static constexpr int epi_warps = 4 * parts;
-    static constexpr int threads = 64 + 32 * epi_warps;                  // warp 0 TMA, warp 1 MMA, the rest epilogue
-    static constexpr int smem = stages * stage_bytes + epi_warps * kSlotBytes + 1024 /* barriers */ + 1024 /* alignment */;
-    static constexpr uint32_t tmem_cols = 2 * kRows;
-    static constexpr uint32_t idesc = tc::idesc_s8(2 * kHalf, kRows);
-};
+constexpr int kEpiParts = 4;                     // epilogue warps per quarter of the TMEM lanes
+constexpr int kEpiWarps = 4 * kEpiParts;
+constexpr int kPairThreads = 64 + 32 * kEpiWarps;    // warp 0 TMA, warp 1 MMA, the rest epilogue
+constexpr int kABytes = kHalf * kBK8;
+constexpr int kMaxRows = 256, kRowStep = 32;     // rows of y per tile (MMA N)
+constexpr int kMaxStages = kRingBytes / (kABytes + kRowStep / 2 * kBK8);
+constexpr int kPairSmem = kRingBytes + kEpiWarps * kSlotBytes + 1024 /* barriers */ + 1024 /* alignment */;
+constexpr uint32_t kTmemCols = 2 * kMaxRows;
 
 __device__ __forceinline__ void mma_pair_s8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -164,47 +352,49 @@ __device__ __forceinline__ void mma_pair_s8(uint32_t d_tmem, uint64_t a_desc, ui
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-template <typename O, int kRows>
-__global__ void __launch_bounds__(Tile<kRows>::threads, 1)
+// Tiles of 2 kHalf channels (MMA M) x tile_rows rows of y (MMA N).
+template <typename O>
+__global__ void __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q,
-                const __grid_constant__ CUtensorMap map_y, int rows, int n, int k_dim, const float *__restrict__ q_scale,
+                const __grid_constant__ CUtensorMap map_y, int tile_rows, int rows, int n, int k_dim, const float *__restrict__ q_scale,
                 const float *__restrict__ w_scale, const float *__restrict__ bias, O *__restrict__ y, int64_t ld_y, int n_tma,
                 int *__restrict__ status) {
-    using S = Tile<kRows>;
     extern __shared__ unsigned char smem_raw[];
+    const int stage_bytes = kABytes + tile_rows / 2 * kBK8, stages = kRingBytes / stage_bytes;
+    const uint32_t idesc = tc::idesc_s8(2 * kHalf, tile_rows);
     const uint32_t raw = (uint32_t)__cvta_generic_to_shared(smem_raw);
     const uint32_t ring = (raw + 1023u) & ~1023u;                        // stage s: w half, then q half
-    const uint32_t staging = ring + S::stages * S::stage_bytes;          // a slot per epilogue warp
-    const uint32_t bars = staging + S::epi_warps * kSlotBytes;
+    const uint32_t staging = ring + kRingBytes;          // a slot per epilogue warp
+    const uint32_t bars = staging + kEpiWarps * kSlotBytes;
     auto full = [&](int s) { return bars + 8u * s; };
-    auto empty = [&](int s) { return bars + 8u * (S::stages + s); };
-    auto tfull = [&](int b) { return bars + 8u * (2 * S::stages + b); };
-    auto tempty = [&](int b) { return bars + 8u * (2 * S::stages + 2 + b); };
-    const uint32_t tmem_slot = bars + 8u * (2 * S::stages + 4);
+    auto empty = [&](int s) { return bars + 8u * (kMaxStages + s); };
+    auto tfull = [&](int b) { return bars + 8u * (2 * kMaxStages + b); };
+    auto tempty = [&](int b) { return bars + 8u * (2 * kMaxStages + 2 + b); };
+    const uint32_t tmem_slot = bars + 8u * (2 * kMaxStages + 4);
     unsigned char *const slot_ptr = smem_raw + (tmem_slot - raw);
 
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_rank();
     const int n_kb = (k_dim + kBK8 - 1) / kBK8;
     const int m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf);
-    const int total = m_tiles * ((rows + kRows - 1) / kRows);
+    const int total = m_tiles * ((rows + tile_rows - 1) / tile_rows);
     const int first = (int)tc::cluster_id(), step = (int)tc::cluster_count();
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::stages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             tc::bar_init(full(s), 1);
             tc::bar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
             tc::bar_init(tfull(b), 1);
-            tc::bar_init(tempty(b), 2 * S::epi_warps);
+            tc::bar_init(tempty(b), 2 * kEpiWarps);
         }
         asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
         asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(&map_q)) : "memory");
     }
     if (warp == 0) {                                                     // warp 0 of both CTAs allocates
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(S::tmem_cols)
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(tmem_slot), "r"(kTmemCols)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
     }
@@ -219,7 +409,7 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
         int s = 0, use = 0;
         bool ok = true;
         for (int t = first; t < total && ok; t += step) {
-            const int m0 = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf, i0 = (t / m_tiles) * kRows + (int)rank * (kRows / 2);
+            const int m0 = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf, i0 = (t / m_tiles) * tile_rows + (int)rank * (tile_rows / 2);
             for (int kb = 0; kb < n_kb; ++kb) {
                 if (use > 0 && !__all_sync(0xffffffffu, tc::wait_bar(empty(s), (use - 1) & 1, status))) {
                     if (issuer) tc::fail(status, 1);
@@ -227,17 +417,17 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
                     break;
                 }
                 if (issuer) {
-                    const uint32_t a_dst = ring + s * S::stage_bytes;
-                    if (rank == 0) tc::bar_expect_tx(full(s), 2 * S::stage_bytes);
+                    const uint32_t a_dst = ring + s * stage_bytes;
+                    if (rank == 0) tc::bar_expect_tx(full(s), 2 * stage_bytes);
                     tc::tma_load_pair(a_dst, &map_w, kb * kBK8, m0, leader_bars + 8u * s);
-                    tc::tma_load_pair(a_dst + S::a_bytes, &map_q, kb * kBK8, i0, leader_bars + 8u * s);
+                    tc::tma_load_pair(a_dst + kABytes, &map_q, kb * kBK8, i0, leader_bars + 8u * s);
                 }
                 __syncwarp();
-                if (++s == S::stages) s = 0, ++use;
+                if (++s == stages) s = 0, ++use;
             }
         }
     } else if (warp == 1 && rank == 0) {                                 // MMA issuer (leader): the whole warp, so that
-        int it = 0, ti = 0;                                              // its state is uniform; one lane issues
+        int s = 0, use = 0, ti = 0;                                      // its state is uniform; one lane issues
         bool ok = true;
         const bool issuer = tc::elect_one();
         for (int t = first; t < total && ok; t += step, ++ti) {
@@ -247,53 +437,57 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const uint32_t d = tmem + (uint32_t)(b * kRows);
-            for (int kb = 0; kb < n_kb; ++kb, ++it) {
-                const int s = it % S::stages, use = it / S::stages;
+            const uint32_t d = tmem + (uint32_t)(b * kMaxRows);
+            for (int kb = 0; kb < n_kb; ++kb) {
                 if (!__all_sync(0xffffffffu, tc::wait_bar(full(s), use & 1, status))) {
                     if (issuer) tc::fail(status, 4);
                     ok = false;
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-                const uint32_t a_src = ring + s * S::stage_bytes;
-                const uint64_t a_desc = tc::smem_desc(a_src), b_desc = tc::smem_desc(a_src + S::a_bytes);
+                const uint32_t a_src = ring + s * stage_bytes;
+                const uint64_t a_desc = tc::smem_desc(a_src), b_desc = tc::smem_desc(a_src + kABytes);
                 // the last k block takes only the 32-wide steps that hold data; the others would add zero fill
                 const int nj = min(kBK8 / kMmaK8, (k_dim - kb * kBK8 + kMmaK8 - 1) / kMmaK8);
                 if (issuer) {
 #pragma unroll
                     for (int j = 0; j < kBK8 / kMmaK8; ++j)              // a step of 32 bytes: 2 in the descriptor's units
-                        if (j < nj) mma_pair_s8(d, a_desc + 2 * j, b_desc + 2 * j, S::idesc, (kb > 0 || j > 0) ? 1u : 0u);
+                        if (j < nj) mma_pair_s8(d, a_desc + 2 * j, b_desc + 2 * j, idesc, (kb > 0 || j > 0) ? 1u : 0u);
                     tc::commit_both(empty(s));                           // the stage is free in both CTAs once these
                     if (kb == n_kb - 1) tc::commit_both(tfull(b));       // MMAs have read it; the accumulator is complete
                 }
                 __syncwarp();
+                if (++s == stages) s = 0, ++use;
             }
         }
     } else if (warp >= 2) {                                              // epilogue (both CTAs)
-        const int quarter = warp & 3, part = (warp - 2) >> 2;            // lanes, and share of the tile's rows
-        constexpr int kPart = kRows / S::parts;
+        // lanes 32 quarter .. + 31; of the tile's 32-row chunks every kEpiParts-th
+        const int quarter = warp & 3, part = (warp - 2) >> 2, chunks = tile_rows / 32;
+        constexpr int kChunks = kMaxRows / 32 / kEpiParts;
         const uint32_t leader_tempty0 = tc::map_to(tempty(0), 0), leader_tempty1 = tc::map_to(tempty(1), 0);
         int ti = 0;
         for (int t = first; t < total; t += step, ++ti) {
             const int b = ti & 1, use_b = ti >> 1;
-            const int m = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf + quarter * 32 + lane, i0 = (t / m_tiles) * kRows + part * kPart;
-            // this tile's scales, fetched while its products run: lane l holds those of rows 32 c + l
+            const int m = (t % m_tiles) * 2 * kHalf + (int)rank * kHalf + quarter * 32 + lane, i0 = (t / m_tiles) * tile_rows + part * 32;
+            // this tile's scales, fetched while its products run: lane l holds its chunks' l-th rows'
             const float ws = m < n ? w_scale[m] : 0.f, bm = m < n && bias ? bias[m] : 0.f;
-            float qs[kPart / 32];
+            float qs[kChunks];
 #pragma unroll
-            for (int c = 0; c < kPart / 32; ++c) qs[c] = i0 + c * 32 + lane < rows ? q_scale[i0 + c * 32 + lane] : 0.f;
+            for (int c = 0; c < kChunks; ++c) {
+                const int i = i0 + c * kEpiParts * 32 + lane;
+                qs[c] = part + c * kEpiParts < chunks && i < rows ? q_scale[i] : 0.f;
+            }
             if (!__all_sync(0xffffffffu, tc::wait_bar(tfull(b), use_b & 1, status))) {
                 if (lane == 0) tc::fail(status, 8);
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll
-            for (int c = 0; c < kPart / 32; ++c) {
-                const int i = i0 + c * 32, left = rows - i;
-                if (left <= 0) break;                                    // uniform over the warp
+            for (int c = 0; c < kChunks; ++c) {
+                const int i = i0 + c * kEpiParts * 32, left = rows - i;
+                if (part + c * kEpiParts >= chunks || left <= 0) break;  // uniform over the warp
                 uint32_t r[32];
-                tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * kRows + part * kPart + c * 32), r);
+                tc::tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * kMaxRows + (part + c * kEpiParts) * 32), r);
                 tc::tmem_wait_ld();
                 O v[32];
 #pragma unroll
@@ -334,7 +528,7 @@ __global__ void __launch_bounds__(Tile<kRows>::threads, 1)
     tc::cluster_sync();                                                  // both CTAs are done with TMEM and barriers
     if (warp == 0) {
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(S::tmem_cols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
     }
 }
 
@@ -366,19 +560,18 @@ int device_pairs() {
     return pairs[dev];
 }
 
-template <typename O, int kRows>
-void launch_pairs(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w,
+template <typename O>
+void launch_pairs(int tile_rows, int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w,
                   int64_t ld_w, const float *w_scale, const float *bias, O *y, int64_t ld_y, int *status, cudaStream_t s) {
-    using S = Tile<kRows>;
     CUtensorMap map_w, map_q, map_y;
     tc::encode_operand_s8(&map_w, w, n, k, ld_w, kHalf);
-    tc::encode_operand_s8(&map_q, q, rows, k, ld_q, kRows / 2);
+    tc::encode_operand_s8(&map_q, q, rows, k, ld_q, (uint32_t)tile_rows / 2);
     // the channels that TMA stores: all but the last few, or none where y's rows do not start on 16 bytes
     const int unit = 16 / (int)sizeof(O);
     const int n_tma = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && ld_y % unit == 0 ? (int)n / unit * unit : 0;
     if (n_tma) encode_result(&map_y, y, rows, n_tma, ld_y);
     else std::memset(&map_y, 0, sizeof(map_y));
-    const int64_t total = (n + 2 * kHalf - 1) / (2 * kHalf) * ((rows + kRows - 1) / kRows);
+    const int64_t total = (n + 2 * kHalf - 1) / (2 * kHalf) * ((rows + tile_rows - 1) / tile_rows);
     AFB_CHECK(total < (1LL << 31), "too many rows for one launch");
     const int64_t pairs = std::min<int64_t>(total, device_pairs());
     cudaLaunchConfig_t cfg = {};
@@ -388,14 +581,28 @@ void launch_pairs(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t l
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
-    cfg.blockDim = dim3(S::threads, 1, 1);
-    cfg.dynamicSmemBytes = S::smem;
+    cfg.blockDim = dim3(kPairThreads, 1, 1);
+    cfg.dynamicSmemBytes = kPairSmem;
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O, kRows>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem));
-    AFB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<O, kRows>, map_w, map_q, map_y, (int)rows, (int)n, (int)k, q_scale, w_scale,
+    AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    AFB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<O>, map_w, map_q, map_y, tile_rows, (int)rows, (int)n, (int)k, q_scale, w_scale,
                                 bias, y, ld_y, n_tma, status));
+}
+
+// Rows of y per tile: the fewest rounds of tiles times the time of one, which is near proportional to 128 + r: 3.3,
+// 4.2, 5.5 and 6.7 us a round at r = 64, 128, 192 and 256 and k = 2333.  1,120 x 2333 -> 4171 takes 17.0 us with the
+// 160 rows that this gives and 19.3 with 256, which are the best for large products.
+int pick_tile_rows(int64_t rows, int64_t n) {
+    const int64_t m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf), pairs = device_pairs();
+    int best = kMaxRows;
+    int64_t best_cost = INT64_MAX;
+    for (int r = kMaxRows; r >= kRowStep; r -= kRowStep) {
+        const int64_t cost = (m_tiles * ((rows + r - 1) / r) + pairs - 1) / pairs * (128 + r);
+        if (cost < best_cost) best = r, best_cost = cost;
+    }
+    return best;
 }
 
 void check_rows16(const void *p, int64_t ld, const char *what) {
@@ -408,10 +615,20 @@ void quantize(int64_t rows, int64_t k, int type, const void *x, int64_t ld_x, in
         using T = decltype(t);
         const T *src = static_cast<const T *>(x);
         if (x_trans) {
-            const int64_t blocks = (rows + kColRows - 1) / kColRows;
+            const int64_t blocks = (rows + kColRows - 1) / kColRows * kColCluster;
+            AFB_CHECK(blocks < (1LL << 31), "too many rows for one launch");
             quantize_columns_kernel<T><<<(unsigned)blocks, 32 * kColWarps, 0, s>>>(rows, k, src, ld_x, norm, q, ld_q, scale);
         } else {
-            quantize_rows_kernel<T><<<(unsigned)rows, kRowThreads, 0, s>>>(k, src, ld_x, norm, q, ld_q, scale);
+            // as few pieces a thread as hold the row wherever it starts
+            auto go = [&](auto p) {
+                quantize_rows_kernel<T, decltype(p)::value><<<(unsigned)rows, kRowThreads, 0, s>>>(k, src, ld_x, norm, q, ld_q, scale);
+            };
+            const int64_t pieces = (k + 16 + kRowThreads * Piece<T>::kPer - 1) / (kRowThreads * Piece<T>::kPer);
+            if (pieces <= 1) go(std::integral_constant<int, 1>{});
+            else if (pieces <= 2) go(std::integral_constant<int, 2>{});
+            else if (pieces <= 3) go(std::integral_constant<int, 3>{});
+            else if (pieces <= 5) go(std::integral_constant<int, 5>{});
+            else go(std::integral_constant<int, kRowPieces>{});
         }
     });
     AFB_LAUNCHED();
@@ -419,29 +636,15 @@ void quantize(int64_t rows, int64_t k, int type, const void *x, int64_t ld_x, in
 
 void matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w, int64_t ld_w,
             const float *w_scale, const float *bias, void *y, int y_type, int64_t ld_y, int *status, cudaStream_t s) {
-    if (rows > kDotRows) {
-        with_type(y_type, [&](auto t) {
-            using O = decltype(t);
-            O *out = static_cast<O *>(y);
-            // the tile that takes the fewest rounds of its size; the wide one moves the fewest bytes a product
-            const int64_t m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf), pairs = device_pairs();
-            auto cost = [&](int64_t r, int64_t unit) { return ((m_tiles * ((rows + r - 1) / r) + pairs - 1) / pairs) * unit; };
-            const int64_t c256 = cost(256, 32), c128 = cost(128, 24), c64 = cost(64, 20);
-            auto go = [&](auto tile) { launch_pairs<O, decltype(tile)::value>(rows, n, k, q, ld_q, q_scale, w, ld_w, w_scale, bias, out, ld_y, status, s); };
-            if (c256 <= c128 && c256 <= c64) go(std::integral_constant<int, 256>{});
-            else if (c128 <= c64) go(std::integral_constant<int, 128>{});
-            else go(std::integral_constant<int, 64>{});
-        });
+    if (few_rows(rows, k)) {
+        launch_dot<int8_t, false>(rows, n, k, q, ld_q, 1, Norm{}, q_scale, w, ld_w, w_scale, bias, y, y_type, ld_y, s);
         return;
     }
-    const dim3 grid((unsigned)((n + kDotWarps - 1) / kDotWarps), (unsigned)((rows + kDotRows - 1) / kDotRows));
-    AFB_CHECK(grid.y < 65536, "too many rows for one launch");
     with_type(y_type, [&](auto t) {
         using O = decltype(t);
-        dot_kernel<O><<<grid, 32 * kDotWarps, 0, s>>>(rows, n, (int)k, q, ld_q, q_scale, w, ld_w, w_scale, bias,
-                                                      static_cast<O *>(y), ld_y);
+        launch_pairs<O>(pick_tile_rows(rows, n), rows, n, k, q, ld_q, q_scale, w, ld_w, w_scale, bias, static_cast<O *>(y), ld_y,
+                        status, s);
     });
-    AFB_LAUNCHED();
 }
 
 // Rows of the quantised matrices in the workspace: a k-block of 128 bytes is then one line of L2 and not two.
@@ -525,11 +728,20 @@ int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, const void *
         check_source(rows, k, x_type, x, ld_x, x_trans, mean, var);
         check_product(n, k, w, ld_w, w_scale, y, y_type, ld_y);
         AFB_CHECK(workspace && workspace_bytes >= afb_int8_linear_workspace(rows, k), "workspace too small (afb_int8_linear_workspace)");
+        const Norm norm{mean, var, eps, clip};
+        if (few_rows(rows, k)) {
+            with_type(x_type, [&](auto t) {
+                using T = decltype(t);
+                launch_dot<T, true>(rows, n, k, static_cast<const T *>(x), x_trans ? 1 : ld_x, x_trans ? ld_x : 1, norm, nullptr, w,
+                                    ld_w, w_scale, bias, y, y_type, ld_y, as_stream(stream));
+            });
+            return;
+        }
         char *ws = reinterpret_cast<char *>((reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255));
         int8_t *q = reinterpret_cast<int8_t *>(ws);
         float *scale = reinterpret_cast<float *>(ws + align256((size_t)rows * round128(k)));
         const cudaStream_t s = as_stream(stream);
-        quantize(rows, k, x_type, x, ld_x, x_trans, Norm{mean, var, eps, clip}, q, round128(k), scale, s);
+        quantize(rows, k, x_type, x, ld_x, x_trans, norm, q, round128(k), scale, s);
         matmul(rows, n, k, q, round128(k), scale, w, ld_w, w_scale, bias, y, y_type, ld_y, status, s);
     });
 }
