@@ -7,8 +7,11 @@ with the reason.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
+
+import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libafb.so")
@@ -127,3 +130,16 @@ def check(code: int) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(load(), name)(*args))
+
+
+_here = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which ``device`` is the current CUDA device; nothing to do, and no cost, where it is already."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def stream_of(device: torch.device) -> int:
+    """The cudaStream_t of ``device``'s current stream."""
+    return torch._C._cuda_getCurrentRawStream(device.index)

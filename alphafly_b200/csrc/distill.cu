@@ -12,6 +12,7 @@
 //       dloss / ds_j = T (q_j - p_j)  in C,   T q_j (1 - p_rest / q_rest)  outside C,  0 outside the support.
 //   The shares of C and of the rest come from the log odds d = lse(C) - lse(rest) as log share(rest) =
 //   -log(1 + exp(d)), so that neither the loss nor the gradient takes a difference of nearly equal sums.
+#include <cfloat>
 #include <cmath>
 
 #include "dtypes.cuh"
@@ -20,6 +21,7 @@ namespace afb {
 namespace {
 
 constexpr float kInf = __builtin_huge_valf();
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 256;                    // largest k
@@ -117,13 +119,14 @@ __device__ __forceinline__ unsigned long long key_of(unsigned order, int move) {
     return ((unsigned long long)order << 32) | (unsigned)~move;
 }
 
-// The k-th largest of the shared group maxima, in warp 0: bit by bit, the largest value that k of them reach.
+// The k-th largest of the shared group maxima to 16 bits, rounded down, in warp 0: bit by bit, the largest value that k
+// of them reach.  A bound some 2^-7 lower lets few more candidates in than the exact one.
 __device__ unsigned kth_of_groups(const unsigned *group, int k) {
     unsigned mine[kGroups / 32];
 #pragma unroll
     for (int g = 0; g < kGroups / 32; ++g) mine[g] = group[g * 32 + (threadIdx.x & 31)];
     unsigned t = 0u;
-    for (int b = 31; b >= 0; --b) {
+    for (int b = 31; b >= 16; --b) {
         const unsigned probe = t | (1u << b);
         int c = 0;
 #pragma unroll
@@ -229,29 +232,171 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
             if (o && key_of(o, mv) < last) sum += expf((value_of(o) - m) * inv_t);
         }
     sum = block_reduce(sum, sh.scratch, 0.f, Sum());
-    if (threadIdx.x == 0) *log_rest = m > -kInf ? m * inv_t + logf(sum) : -kInf;
+    if (threadIdx.x == 0) *log_rest = m > -kInf && m < kInf ? m * inv_t + logf(sum) : m;
 }
 
+// The rows' listed moves: all entries are at hand in shared memory.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) top_kernel(int64_t n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
-                                                       const int64_t *__restrict__ list, const uint8_t *__restrict__ valid,
-                                                       int n_listed, float *__restrict__ values, int64_t *__restrict__ moves,
-                                                       float *__restrict__ log_rest) {
+__global__ void __launch_bounds__(kThreads) top_listed_kernel(int64_t n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
+                                                              const int64_t *__restrict__ list, const uint8_t *__restrict__ valid,
+                                                              int n_listed, float *__restrict__ values, int64_t *__restrict__ moves,
+                                                              float *__restrict__ log_rest) {
     extern __shared__ unsigned dynamic[];
     __shared__ TopShared sh;
     const int64_t i = blockIdx.x;
     const T *row = logits + i * ld;
-    if (list) {
-        const int n_words = (int)((n_moves + 31) / 32);
-        int *listed = reinterpret_cast<int *>(dynamic + n_words);
-        float *at = reinterpret_cast<float *>(listed + n_listed);
-        read_list(list + i * n_listed, valid + i * n_listed, n_listed, n_moves, row, dynamic, n_words, listed, at);
-        select_top(sh, n_listed, k, inv_t, [&](int e, unsigned &o, int &m) { m = listed[e]; o = m < 0 ? 0u : order_of(at[e]); },
-                   values + i * k, moves + i * k, log_rest + i);
-    } else {
-        select_top(sh, (int)n_moves, k, inv_t, [&](int e, unsigned &o, int &m) { o = order_of(to_float(row[e])); m = e; }, values + i * k,
-                   moves + i * k, log_rest + i);
+    const int n_words = (int)((n_moves + 31) / 32);
+    int *listed = reinterpret_cast<int *>(dynamic + n_words);
+    float *at = reinterpret_cast<float *>(listed + n_listed);
+    read_list(list + i * n_listed, valid + i * n_listed, n_listed, n_moves, row, dynamic, n_words, listed, at);
+    select_top(sh, n_listed, k, inv_t, [&](int e, unsigned &o, int &m) { m = listed[e]; o = m < 0 ? 0u : order_of(at[e]); },
+               values + i * k, moves + i * k, log_rest + i);
+}
+
+// 2^x; below 2^-126 it is 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+    return y;
+}
+
+constexpr int kPerThread = 4;                    // candidates of a thread that ranks
+constexpr int kRanked = 32 * kPerThread;         // as many as one warp ranks by itself
+static_assert(kCandidates <= kThreads * kPerThread, "the block ranks all candidates");
+
+// All moves of a row: one CTA per row, P pieces a thread in registers (P = 0: any length, the row is read twice, the
+// second time from cache).  One pass takes the groups' maxima, one collects the moves at or above the bound and sums
+// the exponentials of the others relative to it; one warp ranks the candidates.
+template <typename T, int P>
+__global__ void __launch_bounds__(kThreads) top_kernel(int n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
+                                                       float *__restrict__ values, int64_t *__restrict__ moves,
+                                                       float *__restrict__ log_rest) {
+    constexpr int kPer = Piece<T>::kPer;
+    __shared__ TopShared sh;
+    const int64_t i = blockIdx.x;
+    const T *row = logits + i * ld;
+    const int lead = lead_of(row), lane = threadIdx.x & 31;
+    const T nothing = from_float<T>(-kInf);
+    Piece<T> mine[P ? P : 1];
+    if (P)
+#pragma unroll
+        for (int p = 0; p < P; ++p) mine[p] = load_piece(row, (int64_t)(p * kThreads + threadIdx.x) * kPer - lead, n_moves, nothing);
+    // f(value, move) of this thread's moves; NaN comes as -inf
+    auto each = [&](auto &&f) {
+        if constexpr (P > 0) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const int at = (p * kThreads + (int)threadIdx.x) * kPer - lead;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) f(fmaxf(to_float(mine[p].e[e]), -kInf), at + e, e & 1);
+            }
+        } else {
+            for (int at = (int)threadIdx.x * kPer - lead; at < n_moves; at += kThreads * kPer) {
+                const Piece<T> v = load_piece(row, at, n_moves, nothing);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) f(fmaxf(to_float(v.e[e]), -kInf), at + e, e & 1);
+            }
+        }
+    };
+    float best[2] = {-kInf, -kInf};
+    each([&](float v, int, int half) { best[half] = fmaxf(best[half], v); });
+    sh.group[threadIdx.x] = order_of(best[0]);
+    sh.group[threadIdx.x + kThreads] = order_of(best[1]);
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const unsigned t = kth_of_groups(sh.group, k);
+        // at least the lowest finite value, so that -inf stays below it
+        if (lane == 0) sh.bound = max(t, order_of(-FLT_MAX));
     }
+    __syncthreads();
+    const float bound = value_of(sh.bound), c = inv_t * kLog2e;
+    float below = 0.f;
+    each([&](float v, int m, int) {
+        if (v >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kCandidates) sh.cand[at] = key_of(order_of(v), m);
+        } else {
+            below += exp2_fast((v - bound) * c);
+        }
+    });
+    below = warp_reduce(below, Sum());
+    if (lane == 0) sh.scratch[threadIdx.x >> 5] = below;
+    __syncthreads();
+    const int found = sh.count;
+    values += i * k;
+    moves += i * k;
+    if (found > kCandidates) {                   // many equal values at the bound
+        __syncthreads();                         // all have read the count
+        select_top(sh, n_moves, k, inv_t, [&](int e, unsigned &o, int &m) { o = order_of(to_float(row[e])); m = e; }, values, moves,
+                   log_rest + i);
+        return;
+    }
+    below = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) below += sh.scratch[w];
+    // `step` threads, t of them this one, rank the candidates (how many are larger) and close the row
+    auto close = [&](int t, int step, auto &&reduce) {
+        unsigned long long key[kPerThread];
+        int rank[kPerThread];
+        const int used = (found + step - 1) / step;
+#pragma unroll
+        for (int u = 0; u < kPerThread; ++u) {
+            key[u] = u * step + t < found ? sh.cand[u * step + t] : 0ull;
+            rank[u] = 0;
+        }
+        for (int d = 0; d < found; ++d) {
+            const unsigned long long other = sh.cand[d];
+#pragma unroll
+            for (int u = 0; u < kPerThread; ++u)
+                if (u < used) rank[u] += other > key[u];
+        }
+        float ref = -kInf;                       // the largest candidate that is not among the k
+#pragma unroll
+        for (int u = 0; u < kPerThread; ++u) {
+            if (u * step + t >= found) break;
+            const float v = value_of((unsigned)(key[u] >> 32));
+            if (rank[u] < k) {
+                values[rank[u]] = v;
+                moves[rank[u]] = (int64_t) ~(unsigned)key[u];
+            } else {
+                ref = fmaxf(ref, v);
+            }
+        }
+        for (int r = found + t; r < k; r += step) {
+            values[r] = -kInf;
+            moves[r] = -1;
+        }
+        float left = 0.f, out = -kInf;
+        if (found > k) {                         // ref is at least the bound: the largest of all that are left
+            ref = reduce(ref, -kInf, Max());
+#pragma unroll
+            for (int u = 0; u < kPerThread; ++u)
+                if (u * step + t < found && rank[u] >= k) left += exp2_fast((value_of((unsigned)(key[u] >> 32)) - ref) * c);
+            left = reduce(left, 0.f, Sum());
+            out = ref * inv_t + logf(left + below * exp2_fast((bound - ref) * c));
+        } else if (found == k && below > 1e-25f) {
+            out = bound * inv_t + logf(below);
+        } else if (found == k) {                 // all that is left lies far below the bound, or nothing is
+            for (int e = t; e < n_moves; e += step) {
+                const float v = to_float(row[e]);
+                if (v < bound) ref = fmaxf(ref, v);
+            }
+            ref = reduce(ref, -kInf, Max());
+            if (ref > -kInf)
+                for (int e = t; e < n_moves; e += step) {
+                    const float v = to_float(row[e]);
+                    if (v < bound) left += exp2_fast((v - ref) * c);
+                }
+            left = reduce(left, 0.f, Sum());
+            if (ref > -kInf) out = ref * inv_t + logf(left);
+        }
+        if (t == 0) log_rest[i] = ref == kInf ? kInf : out;           // -inf for fewer than k moves
+    };
+    if (found > kRanked)
+        close((int)threadIdx.x, kThreads, [&](float x, float unit, auto &&f) { return block_reduce(x, sh.scratch, unit, f); });
+    else if (threadIdx.x < 32)
+        close(lane, 32, [&](float x, float, auto &&f) { return warp_reduce(x, f); });
 }
 
 __device__ __forceinline__ float softplus(float d) { return fmaxf(d, 0.f) + log1pf(expf(-fabsf(d))); }
@@ -464,13 +609,29 @@ int afb_top_logits(int64_t rows, int64_t n_moves, int type, const void *logits, 
         check_rows(rows, n_moves, type, logits, ld, k, temperature, legal, valid, n_listed);
         if (rows == 0) return;
         AFB_CHECK(values && moves && log_rest, "NULL pointer");
-        const size_t shared = legal ? (size_t)((n_moves + 31) / 32) * 4 + (size_t)n_listed * 8 : 0;
+        const cudaStream_t s = as_stream(stream);
+        const float inv_t = 1.f / temperature;
         with_type(type, [&](auto e) {
             using T = decltype(e);
-            allow_shared(top_kernel<T>, shared);
-            top_kernel<T><<<(unsigned)rows, kThreads, shared, as_stream(stream)>>>(n_moves, static_cast<const T *>(logits), ld, k,
-                                                                                   1.f / temperature, legal, valid, (int)n_listed,
-                                                                                   values, moves, log_rest);
+            const T *x = static_cast<const T *>(logits);
+            if (legal) {
+                const size_t shared = (size_t)((n_moves + 31) / 32) * 4 + (size_t)n_listed * 8;
+                allow_shared(top_listed_kernel<T>, shared);
+                top_listed_kernel<T><<<(unsigned)rows, kThreads, shared, s>>>(n_moves, x, ld, k, inv_t, legal, valid, (int)n_listed,
+                                                                              values, moves, log_rest);
+                return;
+            }
+            // as few pieces a thread as hold a row wherever it starts
+            auto go = [&](auto p) {
+                top_kernel<T, decltype(p)::value><<<(unsigned)rows, kThreads, 0, s>>>((int)n_moves, x, ld, k, inv_t, values, moves, log_rest);
+            };
+            const int64_t span = kThreads * Piece<T>::kPer, pieces = (n_moves + Piece<T>::kPer + span - 1) / span;
+            if (pieces <= 1) go(std::integral_constant<int, 1>{});
+            else if (pieces <= 2) go(std::integral_constant<int, 2>{});
+            else if (pieces <= 3) go(std::integral_constant<int, 3>{});
+            else if (pieces <= 5) go(std::integral_constant<int, 5>{});
+            else if (pieces <= 8) go(std::integral_constant<int, 8>{});
+            else go(std::integral_constant<int, 0>{});
         });
         AFB_LAUNCHED();
     });

@@ -21,6 +21,36 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// 16 bytes of a row: kPer elements.
+template <typename T>
+struct Piece {
+    static constexpr int kPer = 16 / (int)sizeof(T);
+    union {
+        uint4 raw;
+        T e[kPer];
+    };
+    __device__ __forceinline__ Piece() : raw(make_uint4(0u, 0u, 0u, 0u)) {}
+};
+
+// Elements of a row's first 16-byte piece that lie before the row.
+template <typename T>
+__device__ __forceinline__ int lead_of(const T *row) {
+    return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+}
+
+// The piece of a row of n elements that starts at element at (row + at on 16 bytes); what is not of the row is `fill`.
+template <typename T>
+__device__ __forceinline__ Piece<T> load_piece(const T *row, int64_t at, int64_t n, T fill) {
+    Piece<T> v;
+    if (at >= 0 && at + Piece<T>::kPer <= n) {
+        v.raw = __ldg(reinterpret_cast<const uint4 *>(row + at));
+    } else {
+#pragma unroll
+        for (int e = 0; e < Piece<T>::kPer; ++e) v.e[e] = at + e >= 0 && at + e < n ? row[at + e] : fill;
+    }
+    return v;
+}
+
 inline bool known_type(int t) { return t == AFB_T_F32 || t == AFB_T_F16 || t == AFB_T_BF16; }
 inline size_t type_size(int t) { return t == AFB_T_F32 ? 4 : 2; }
 

@@ -66,17 +66,6 @@ struct Norm {
     }
 };
 
-// 16 bytes of x: kPer elements.
-template <typename T>
-struct Piece {
-    static constexpr int kPer = 16 / (int)sizeof(T);
-    union {
-        uint4 raw;
-        T e[kPer];
-    };
-    __device__ __forceinline__ Piece() : raw(make_uint4(0u, 0u, 0u, 0u)) {}
-};
-
 constexpr int kRowThreads = 128;
 constexpr int kRowPieces = 8;                    // most 16-byte pieces a thread keeps
 
@@ -93,7 +82,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int64_t k_di
     __shared__ uint32_t bytes[kSpan / 4];
     const int64_t i = blockIdx.x;
     const T *row = x + i * ld;
-    const int lead = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int lead = lead_of(row);
     if (threadIdx.x == 0) amax = 0u;
     __syncthreads();
     Piece<T> mine[P];
@@ -102,12 +91,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int64_t k_di
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int64_t k = first_of(base, p);
-            mine[p] = Piece<T>();
-            if (k >= 0 && k + kPer <= k_dim) mine[p].raw = __ldg(reinterpret_cast<const uint4 *>(row + k));
-            else if (k < k_dim)
-#pragma unroll
-                for (int e = 0; e < kPer; ++e)
-                    if (k + e >= 0 && k + e < k_dim) mine[p].e[e] = row[k + e];
+            mine[p] = k < k_dim ? load_piece(row, k, k_dim, from_float<T>(0.f)) : Piece<T>();
         }
     };
     auto value = [&](int64_t base, int p, int e) {
@@ -713,7 +697,7 @@ int afb_int8_matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t
 }
 
 size_t afb_int8_linear_workspace(int64_t rows, int64_t k) {
-    if (rows <= 0 || k <= 0) return 0;
+    if (rows <= 0 || k <= 0 || few_rows(rows, k)) return 0;
     return align256((size_t)rows * round128(k)) + align256((size_t)rows * 4) + 256;
 }
 
@@ -727,7 +711,8 @@ int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, const void *
         AFB_CHECK(k >= 1, "k must be positive");
         check_source(rows, k, x_type, x, ld_x, x_trans, mean, var);
         check_product(n, k, w, ld_w, w_scale, y, y_type, ld_y);
-        AFB_CHECK(workspace && workspace_bytes >= afb_int8_linear_workspace(rows, k), "workspace too small (afb_int8_linear_workspace)");
+        const size_t need = afb_int8_linear_workspace(rows, k);
+        AFB_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (afb_int8_linear_workspace)");
         const Norm norm{mean, var, eps, clip};
         if (few_rows(rows, k)) {
             with_type(x_type, [&](auto t) {

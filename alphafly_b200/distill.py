@@ -47,7 +47,7 @@ def _check_logits(logits: torch.Tensor, temperature: float) -> torch.Tensor:
 def _matrix(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device, name: str) -> torch.Tensor:
     if tuple(t.shape) != shape or t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be {dtype} {shape} on the logits' device, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _legal(legal, logits: torch.Tensor):
@@ -66,7 +66,6 @@ def _ptr(t: torch.Tensor | None):
     return t.data_ptr() if t is not None else None
 
 
-@torch.no_grad()
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=None) -> TopLogits:
     """The k (at most 256) largest of each row of ``logits`` (B, moves), equal ones by the lower move; -inf and NaN
     are never taken.  ``legal``: (moves (B, K) int64, valid (B, K) bool), as a ``train.Batch`` holds them, restricts
@@ -79,10 +78,10 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=Non
     moves, valid, listed = _legal(legal, logits)
     out = TopLogits(torch.empty(b, k, dtype=torch.float32, device=dev), torch.empty(b, k, dtype=torch.int64, device=dev),
                     torch.empty(b, dtype=torch.float32, device=dev), float(temperature))
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.call("afb_top_logits", b, n, TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), k, float(temperature),
                   _ptr(moves), _ptr(valid), listed, out.values.data_ptr(), out.moves.data_ptr(), out.log_rest.data_ptr(),
-                  torch.cuda.current_stream(dev).cuda_stream)
+                  _lib.stream_of(dev))
     return out
 
 
@@ -110,11 +109,11 @@ class _Distillation(torch.autograd.Function):
         temperature, scale = args
         b, n = logits.shape
         dev = logits.device
-        with torch.cuda.device(dev):
+        with _lib.on_device(dev):
             _lib.call("afb_distill_loss", b, n, TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), values.shape[1],
                       values.data_ptr(), moves.data_ptr(), _ptr(log_rest), temperature, _ptr(legal_moves), _ptr(legal_valid),
                       legal_moves.shape[1] if legal_moves is not None else 0, _ptr(weight), scale, _ptr(upstream), step,
-                      int(skip_ones), _ptr(rows), _ptr(total), _ptr(grad), n, torch.cuda.current_stream(dev).cuda_stream)
+                      int(skip_ones), _ptr(rows), _ptr(total), _ptr(grad), n, _lib.stream_of(dev))
 
     @staticmethod
     @torch.autograd.function.once_differentiable

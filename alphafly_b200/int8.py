@@ -61,7 +61,7 @@ def _vector(t: torch.Tensor | None, n: int, device, name: str) -> torch.Tensor |
         return None
     if t.shape != (n,) or t.dtype != torch.float32 or t.device != device:
         raise ValueError(f"{name} must be float32 ({n},) on x's device")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def empty_rows(rows: int, k: int, device) -> torch.Tensor:
@@ -70,7 +70,6 @@ def empty_rows(rows: int, k: int, device) -> torch.Tensor:
     return torch.empty(rows, max(-(-k // 128) * 128, 128), dtype=torch.int8, device=device)[:, :k]
 
 
-@torch.no_grad()
 def quantize(x: torch.Tensor, norm=None) -> tuple[torch.Tensor, torch.Tensor]:
     """x (rows, k) float32, float16 or bfloat16, contiguous or transposed -> (q int8 (rows, k), scale float32
     (rows,)) with x ~ q * scale[:, None].  ``norm``: a ``RunningNorm`` whose running statistics are applied to x
@@ -80,9 +79,9 @@ def quantize(x: torch.Tensor, norm=None) -> tuple[torch.Tensor, torch.Tensor]:
     x, ld, trans = _source(x)
     q = empty_rows(rows, k, x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
+    with _lib.on_device(x.device):
         _lib.call("afb_quantize_rows", rows, k, TYPES[x.dtype], x.data_ptr(), ld, trans, *_norm_args(norm), q.data_ptr(),
-                  q.stride(0), scale.data_ptr(), torch.cuda.current_stream(x.device).cuda_stream)
+                  q.stride(0), scale.data_ptr(), _lib.stream_of(x.device))
     return q, scale
 
 
@@ -95,17 +94,16 @@ def _result(rows: int, n: int, k: int, w, w_scale, bias, out_dtype, device):
     # rows on 16 bytes let the kernel store through TMA; on 128, where that is little padding, its stores are whole lines
     size = 4 if out_dtype == torch.float32 else 2
     unit = (128 if n * size >= 1024 else 16) // size
-    y = torch.empty(rows, -(-n // unit) * unit, dtype=out_dtype, device=device)[:, :n]
+    y = torch.empty_strided((rows, n), (-(-n // unit) * unit, 1), dtype=out_dtype, device=device)
     return w, _vector(w_scale, n, device, "w_scale"), _vector(bias, n, device, "bias"), y
 
 
-def _empty_sum(y: torch.Tensor, bias, x_scale=None) -> torch.Tensor:
+def _empty_sum(y: torch.Tensor, bias) -> torch.Tensor:
     """The product over k = 0."""
     y.zero_()
-    return y if bias is None else y.add_(bias.to(y.dtype))
+    return y if bias is None else y.add_(bias.detach().to(y.dtype))
 
 
-@torch.no_grad()
 def int8_matmul(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """(q w^T) * scale[:, None] * w_scale + bias, (rows, n) of ``out_dtype`` (rounded once), a view whose rows start
@@ -122,14 +120,13 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: 
     w, w_scale, bias, y = _result(rows, n, k, w, w_scale, bias, out_dtype, dev)
     if k == 0:
         return _empty_sum(y, bias)
-    with torch.cuda.device(dev):
+    with _lib.on_device(dev):
         _lib.call("afb_int8_matmul", rows, n, k, q.data_ptr(), q.stride(0), scale.data_ptr(), w.data_ptr(), w.stride(0),
                   w_scale.data_ptr(), bias.data_ptr() if bias is not None else None, y.data_ptr(), TYPES[out_dtype], y.stride(0),
-                  _device_status(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
+                  _device_status(dev).data_ptr(), _lib.stream_of(dev))
     return y
 
 
-@torch.no_grad()
 def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None, norm=None,
                 out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """``quantize(x, norm)`` times the quantised weight: x (rows, k) float32, float16 or bfloat16, contiguous or a
@@ -143,10 +140,11 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
         return _empty_sum(y, bias)
     x, ld, trans = _source(x)
     lib = _lib.load()
-    ws = torch.empty(lib.afb_int8_linear_workspace(rows, k), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
+    size = lib.afb_int8_linear_workspace(rows, k)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    with _lib.on_device(dev):
         _lib.check(lib.afb_int8_linear(rows, n, k, TYPES[x.dtype], x.data_ptr(), ld, trans, *_norm_args(norm), w.data_ptr(),
                                        w.stride(0), w_scale.data_ptr(), bias.data_ptr() if bias is not None else None,
-                                       y.data_ptr(), TYPES[out_dtype], y.stride(0), ws.data_ptr(), ws.numel(),
-                                       _device_status(dev).data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
+                                       y.data_ptr(), TYPES[out_dtype], y.stride(0), ws.data_ptr() if size else None, size,
+                                       _device_status(dev).data_ptr(), _lib.stream_of(dev)))
     return y

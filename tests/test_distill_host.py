@@ -48,8 +48,8 @@ def test_int8_product_arguments():
     bad("leading dimension", 12, 8)
     bad("element type", 11, -1)
     _lib.call("afb_int8_matmul", 0, *good[1:])
-    assert _lib.load().afb_int8_linear_workspace(0, 7) == 0 and _lib.load().afb_int8_linear_workspace(3, 7) >= 3 * 16 + 12
-    _raises("workspace too small", "afb_int8_linear", 4, 9, 40, 0, P, 40, 0, None, None, 0.0, 0.0, P, 48, P, None, P, 0, 9, P, 10, None, None)
+    assert _lib.load().afb_int8_linear_workspace(0, 7) == 0 and _lib.load().afb_int8_linear_workspace(300, 7) >= 300 * (16 + 4)
+    _raises("workspace too small", "afb_int8_linear", 400, 9, 40, 0, P, 40, 0, None, None, 0.0, 0.0, P, 48, P, None, P, 0, 9, P, 10, None, None)
 
 
 def test_top_logits_arguments():
