@@ -14,6 +14,7 @@
 //   -log(1 + exp(d)), so that neither the loss nor the gradient takes a difference of nearly equal sums.
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "dtypes.cuh"
 
@@ -27,7 +28,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 256;                    // largest k
 constexpr int kMaxListed = 4096;                // longest list of moves
 constexpr int64_t kMaxMoves = 1 << 20;          // the bitmap of a row's moves fits in shared memory
-constexpr int kGroups = 2 * kThreads;           // at least kMaxTop
+constexpr int kGroups = 512;                    // at least kMaxTop
 constexpr int kCandidates = 1024;
 static_assert(kGroups >= kMaxTop && kCandidates >= kMaxTop, "k groups and k candidates");
 
@@ -53,8 +54,7 @@ __device__ __forceinline__ float block_reduce(float x, float *scratch, float uni
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
     x = unit;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) x = f(x, scratch[w]);
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) x = f(x, scratch[w]);
     return x;
 }
 struct Max {
@@ -69,8 +69,7 @@ __device__ __forceinline__ int block_count(int x, int *scratch) {
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
     x = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) x += scratch[w];
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) x += scratch[w];
     return x;
 }
 
@@ -119,47 +118,60 @@ __device__ __forceinline__ unsigned long long key_of(unsigned order, int move) {
     return ((unsigned long long)order << 32) | (unsigned)~move;
 }
 
-// The k-th largest of the shared group maxima to 16 bits, rounded down, in warp 0: bit by bit, the largest value that k
-// of them reach.  A bound some 2^-7 lower lets few more candidates in than the exact one.
+// A lower bound of the k-th largest of the first G shared group maxima, in warp 0: bit by bit from the first in which they
+// differ, the largest value that k of them reach, until few more than k do.
+template <int G>
 __device__ unsigned kth_of_groups(const unsigned *group, int k) {
-    unsigned mine[kGroups / 32];
+    unsigned mine[G / 32], all = ~0u, any = 0u;
 #pragma unroll
-    for (int g = 0; g < kGroups / 32; ++g) mine[g] = group[g * 32 + (threadIdx.x & 31)];
-    unsigned t = 0u;
-    for (int b = 31; b >= 16; --b) {
-        const unsigned probe = t | (1u << b);
+    for (int g = 0; g < G / 32; ++g) {
+        mine[g] = group[g * 32 + (threadIdx.x & 31)];
+        all &= mine[g];
+        any |= mine[g];
+    }
+    all = __reduce_and_sync(0xffffffffu, all);
+    any = __reduce_or_sync(0xffffffffu, any);
+    if (all == any) return all;
+    unsigned bit = 0x80000000u >> __clz(all ^ any), t = all & ~(2u * bit - 1u);
+    for (int reach = G; bit && reach > k + k / 8; bit >>= 1) {
+        const unsigned probe = t | bit;
         int c = 0;
 #pragma unroll
-        for (int g = 0; g < kGroups / 32; ++g) c += mine[g] >= probe;
-        if (__reduce_add_sync(0xffffffffu, c) >= k) t = probe;
+        for (int g = 0; g < G / 32; ++g) c += mine[g] >= probe;
+        c = __reduce_add_sync(0xffffffffu, c);
+        if (c >= k) t = probe, reach = c;
     }
     return t;
 }
 
 // Selects from `n` entries, get(e, order, move).  A row with too many entries at the bound (many equal values) finds
 // the k-th key itself bit by bit.
-template <typename Get>
+template <int NT, typename Get>
 __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, float *values, int64_t *moves, float *log_rest) {
-    for (int g = threadIdx.x; g < kGroups; g += kThreads) sh.group[g] = 0u;
+    for (int g = threadIdx.x; g < kGroups; g += NT) sh.group[g] = 0u;
     if (threadIdx.x == 0) sh.count = 0;
-    // entry e belongs to group e mod kGroups: a thread's entries fall into two groups
-    unsigned best[2] = {0u, 0u};
-    for (int e = threadIdx.x, h = 0; e < n; e += kThreads, h ^= 1) {
-        unsigned o;
-        int m;
-        get(e, o, m);
-        best[h] = max(best[h], o);
-    }
-    sh.group[threadIdx.x] = best[0];
-    sh.group[threadIdx.x + kThreads] = best[1];
+    // entry e belongs to group e mod kGroups
+    unsigned best[kGroups / NT] = {};
+    for (int e0 = 0; e0 < n; e0 += kGroups)
+#pragma unroll
+        for (int h = 0; h < kGroups / NT; ++h) {
+            const int e = e0 + h * NT + (int)threadIdx.x;
+            if (e >= n) break;
+            unsigned o;
+            int m;
+            get(e, o, m);
+            best[h] = max(best[h], o);
+        }
+#pragma unroll
+    for (int h = 0; h < kGroups / NT; ++h) sh.group[h * NT + threadIdx.x] = best[h];
     __syncthreads();
     if (threadIdx.x < 32) {
-        const unsigned t = kth_of_groups(sh.group, k);
+        const unsigned t = kth_of_groups<kGroups>(sh.group, k);
         if (threadIdx.x == 0) sh.bound = max(t, 1u);                      // 0: fewer than k groups hold a move
     }
     __syncthreads();
     unsigned bound = sh.bound;
-    for (int e = threadIdx.x; e < n; e += kThreads) {
+    for (int e = threadIdx.x; e < n; e += NT) {
         unsigned o;
         int m;
         get(e, o, m);
@@ -175,7 +187,7 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
         for (int b = 63; b >= 0; --b) {
             const unsigned long long probe = t | (1ull << b);
             int c = 0;
-            for (int e = threadIdx.x; e < n; e += kThreads) {
+            for (int e = threadIdx.x; e < n; e += NT) {
                 unsigned o;
                 int m;
                 get(e, o, m);
@@ -186,7 +198,7 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
         __syncthreads();
         if (threadIdx.x == 0) sh.count = 0;
         __syncthreads();
-        for (int e = threadIdx.x; e < n; e += kThreads) {
+        for (int e = threadIdx.x; e < n; e += NT) {
             unsigned o;
             int m;
             get(e, o, m);
@@ -197,7 +209,7 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
     }
     if (threadIdx.x == 0) sh.last = 0ull;
     __syncthreads();
-    for (int c = threadIdx.x; c < found; c += kThreads) {
+    for (int c = threadIdx.x; c < found; c += NT) {
         const unsigned long long key = sh.cand[c];
         int rank = 0;
         for (int d = 0; d < found; ++d) rank += sh.cand[d] > key;
@@ -207,7 +219,7 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
             if (rank == k - 1) sh.last = key;
         }
     }
-    for (int r = found + threadIdx.x; r < k; r += kThreads) {
+    for (int r = found + threadIdx.x; r < k; r += NT) {
         values[r] = -kInf;
         moves[r] = -1;
     }
@@ -216,7 +228,7 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
     const unsigned long long last = sh.last;
     float m = -kInf;
     if (last)
-        for (int e = threadIdx.x; e < n; e += kThreads) {
+        for (int e = threadIdx.x; e < n; e += NT) {
             unsigned o;
             int mv;
             get(e, o, mv);
@@ -225,7 +237,7 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
     m = block_reduce(m, sh.scratch, -kInf, Max());
     float sum = 0.f;
     if (m > -kInf)
-        for (int e = threadIdx.x; e < n; e += kThreads) {
+        for (int e = threadIdx.x; e < n; e += NT) {
             unsigned o;
             int mv;
             get(e, o, mv);
@@ -249,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) top_listed_kernel(int64_t n_moves, c
     int *listed = reinterpret_cast<int *>(dynamic + n_words);
     float *at = reinterpret_cast<float *>(listed + n_listed);
     read_list(list + i * n_listed, valid + i * n_listed, n_listed, n_moves, row, dynamic, n_words, listed, at);
-    select_top(sh, n_listed, k, inv_t, [&](int e, unsigned &o, int &m) { m = listed[e]; o = m < 0 ? 0u : order_of(at[e]); },
+    select_top<kThreads>(sh, n_listed, k, inv_t, [&](int e, unsigned &o, int &m) { m = listed[e]; o = m < 0 ? 0u : order_of(at[e]); },
                values + i * k, moves + i * k, log_rest + i);
 }
 
@@ -260,66 +272,113 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-constexpr int kPerThread = 4;                    // candidates of a thread that ranks
-constexpr int kRanked = 32 * kPerThread;         // as many as one warp ranks by itself
-static_assert(kCandidates <= kThreads * kPerThread, "the block ranks all candidates");
+constexpr int kRanked = 96;                      // candidates that one warp ranks by itself
 
-// All moves of a row: one CTA per row, P pieces a thread in registers (P = 0: any length, the row is read twice, the
-// second time from cache).  One pass takes the groups' maxima, one collects the moves at or above the bound and sums
-// the exponentials of the others relative to it; one warp ranks the candidates.
-template <typename T, int P>
-__global__ void __launch_bounds__(kThreads) top_kernel(int n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
-                                                       float *__restrict__ values, int64_t *__restrict__ moves,
-                                                       float *__restrict__ log_rest) {
-    constexpr int kPer = Piece<T>::kPer;
+// The largest of each of four subsets of a thread's moves (a maximum passes NaN over); 16-bit types two at a time.
+template <typename T>
+struct FourMax {
+    using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    Two two[4];
+    __device__ __forceinline__ FourMax() {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) two[h].x = two[h].y = from_float<T>(-kInf);
+    }
+    __device__ __forceinline__ void add(const Piece<T> &v) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) two[h] = __hmax2(two[h], *reinterpret_cast<const Two *>(&v.e[2 * h]));
+    }
+    __device__ __forceinline__ float get(int h) const { return fmaxf(to_float(two[h].x), to_float(two[h].y)); }
+};
+template <>
+struct FourMax<float> {
+    float one[4] = {-kInf, -kInf, -kInf, -kInf};
+    __device__ __forceinline__ void add(const Piece<float> &v) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) one[h] = fmaxf(one[h], v.e[h]);
+    }
+    __device__ __forceinline__ float get(int h) const { return one[h]; }
+};
+
+// All moves of a row: one CTA per row, of NT threads, P pieces a thread in registers (P = 0: any length, the row is read
+// twice, the second time from cache).  One pass takes the groups' maxima, one collects the moves at or above the bound
+// and sums the exponentials of the others relative to it; one warp ranks the candidates.
+template <typename T, int NT, int P>
+__global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
+                                                 float *__restrict__ values, int64_t *__restrict__ moves,
+                                                 float *__restrict__ log_rest) {
+    constexpr int kPer = Piece<T>::kPer, kChunk = P ? P : 4;             // pieces at hand at once
     __shared__ TopShared sh;
     const int64_t i = blockIdx.x;
     const T *row = logits + i * ld;
     const int lead = lead_of(row), lane = threadIdx.x & 31;
-    const T nothing = from_float<T>(-kInf);
-    Piece<T> mine[P ? P : 1];
-    if (P)
+    Piece<T> mine[kChunk];
+    auto load = [&](int at) {                    // the chunk whose first piece starts at `at`
 #pragma unroll
-        for (int p = 0; p < P; ++p) mine[p] = load_piece(row, (int64_t)(p * kThreads + threadIdx.x) * kPer - lead, n_moves, nothing);
-    // f(value, move) of this thread's moves; NaN comes as -inf
-    auto each = [&](auto &&f) {
-        if constexpr (P > 0) {
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                const int at = (p * kThreads + (int)threadIdx.x) * kPer - lead;
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) f(fmaxf(to_float(mine[p].e[e]), -kInf), at + e, e & 1);
-            }
-        } else {
-            for (int at = (int)threadIdx.x * kPer - lead; at < n_moves; at += kThreads * kPer) {
-                const Piece<T> v = load_piece(row, at, n_moves, nothing);
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) f(fmaxf(to_float(v.e[e]), -kInf), at + e, e & 1);
-            }
-        }
+        for (int p = 0; p < kChunk; ++p) mine[p] = load_piece(row, at + p * NT * kPer, n_moves, from_float<T>(-kInf));
     };
-    float best[2] = {-kInf, -kInf};
-    each([&](float v, int, int half) { best[half] = fmaxf(best[half], v); });
-    sh.group[threadIdx.x] = order_of(best[0]);
-    sh.group[threadIdx.x + kThreads] = order_of(best[1]);
+    const int first = (int)threadIdx.x * kPer - lead, step = kChunk * NT * kPer;
+    FourMax<T> max4;
+    for (int at = first; at < n_moves; at += step) {
+        load(at);
+#pragma unroll
+        for (int p = 0; p < kChunk; ++p) max4.add(mine[p]);
+        if (P) break;
+    }
+    float best[4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) best[h] = max4.get(h);
+    // up to four groups a thread, as many as give k of them a good bound
+    const float most = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+    if (4 * k <= NT) {
+        sh.group[threadIdx.x] = order_of(most);
+    } else if (2 * k <= NT || kGroups == 2 * NT) {
+        sh.group[threadIdx.x] = order_of(fmaxf(best[0], best[2]));
+        sh.group[threadIdx.x + NT] = order_of(fmaxf(best[1], best[3]));
+    } else {
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+            if (h * NT < kGroups) sh.group[h * NT + threadIdx.x] = order_of(best[h]);
+    }
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     if (threadIdx.x < 32) {
-        const unsigned t = kth_of_groups(sh.group, k);
+        const unsigned t = 4 * k <= NT ? kth_of_groups<NT>(sh.group, k)
+                           : 2 * k <= NT || kGroups == 2 * NT ? kth_of_groups<2 * NT>(sh.group, k) : kth_of_groups<kGroups>(sh.group, k);
         // at least the lowest finite value, so that -inf stays below it
         if (lane == 0) sh.bound = max(t, order_of(-FLT_MAX));
     }
     __syncthreads();
     const float bound = value_of(sh.bound), c = inv_t * kLog2e;
+    const float bc = fmaxf(bound * c, -FLT_MAX);
     float below = 0.f;
-    each([&](float v, int m, int) {
-        if (v >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < kCandidates) sh.cand[at] = key_of(order_of(v), m);
-        } else {
-            below += exp2_fast((v - bound) * c);
+    for (int at = first; at < n_moves; at += step) {
+        if (!P) load(at);
+        if (most >= bound) {                     // few threads; the moves are marked first, which keeps the code short
+            constexpr int kPieces = 32 / kPer;   // of a word of marks
+#pragma unroll
+            for (int p0 = 0; p0 < kChunk; p0 += kPieces) {
+                uint32_t marks = 0u;
+#pragma unroll
+                for (int u = 0; u < kPieces && p0 + u < kChunk; ++u)
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e)
+                        if (to_float(mine[p0 + u < kChunk ? p0 + u : 0].e[e]) >= bound) marks |= 1u << (u * kPer + e);
+                for (; marks; marks &= marks - 1) {
+                    const int bit = __ffs((int)marks) - 1, m = at + (p0 + bit / kPer) * NT * kPer + bit % kPer;
+                    const int place = atomicAdd(&sh.count, 1);
+                    if (place < kCandidates) sh.cand[place] = key_of(order_of(to_float(row[m])), m);
+                }
+            }
         }
-    });
+#pragma unroll
+        for (int p = 0; p < kChunk; ++p)
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const float v = to_float(mine[p].e[e]), x = exp2_fast(fmaf(v, c, -bc));
+                if (v < bound) below += x;
+            }
+        if (P) break;
+    }
     below = warp_reduce(below, Sum());
     if (lane == 0) sh.scratch[threadIdx.x >> 5] = below;
     __syncthreads();
@@ -328,32 +387,32 @@ __global__ void __launch_bounds__(kThreads) top_kernel(int n_moves, const T *__r
     moves += i * k;
     if (found > kCandidates) {                   // many equal values at the bound
         __syncthreads();                         // all have read the count
-        select_top(sh, n_moves, k, inv_t, [&](int e, unsigned &o, int &m) { o = order_of(to_float(row[e])); m = e; }, values, moves,
+        select_top<NT>(sh, n_moves, k, inv_t, [&](int e, unsigned &o, int &m) { o = order_of(to_float(row[e])); m = e; }, values, moves,
                    log_rest + i);
         return;
     }
     below = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) below += sh.scratch[w];
+    for (int w = 0; w < NT / 32; ++w) below += sh.scratch[w];
     // `step` threads, t of them this one, rank the candidates (how many are larger) and close the row
-    auto close = [&](int t, int step, auto &&reduce) {
-        unsigned long long key[kPerThread];
-        int rank[kPerThread];
-        const int used = (found + step - 1) / step;
+    auto close = [&](int t, int step, auto per, auto &&reduce) {
+        constexpr int U = decltype(per)::value;  // candidates a thread ranks
+        unsigned long long key[U];
+        int rank[U];
 #pragma unroll
-        for (int u = 0; u < kPerThread; ++u) {
+        for (int u = 0; u < U; ++u) {
             key[u] = u * step + t < found ? sh.cand[u * step + t] : 0ull;
             rank[u] = 0;
         }
+#pragma unroll 4
         for (int d = 0; d < found; ++d) {
             const unsigned long long other = sh.cand[d];
 #pragma unroll
-            for (int u = 0; u < kPerThread; ++u)
-                if (u < used) rank[u] += other > key[u];
+            for (int u = 0; u < U; ++u) rank[u] += other > key[u];
         }
         float ref = -kInf;                       // the largest candidate that is not among the k
 #pragma unroll
-        for (int u = 0; u < kPerThread; ++u) {
+        for (int u = 0; u < U; ++u) {
             if (u * step + t >= found) break;
             const float v = value_of((unsigned)(key[u] >> 32));
             if (rank[u] < k) {
@@ -371,7 +430,7 @@ __global__ void __launch_bounds__(kThreads) top_kernel(int n_moves, const T *__r
         if (found > k) {                         // ref is at least the bound: the largest of all that are left
             ref = reduce(ref, -kInf, Max());
 #pragma unroll
-            for (int u = 0; u < kPerThread; ++u)
+            for (int u = 0; u < U; ++u)
                 if (u * step + t < found && rank[u] >= k) left += exp2_fast((value_of((unsigned)(key[u] >> 32)) - ref) * c);
             left = reduce(left, 0.f, Sum());
             out = ref * inv_t + logf(left + below * exp2_fast((bound - ref) * c));
@@ -393,10 +452,17 @@ __global__ void __launch_bounds__(kThreads) top_kernel(int n_moves, const T *__r
         }
         if (t == 0) log_rest[i] = ref == kInf ? kInf : out;           // -inf for fewer than k moves
     };
-    if (found > kRanked)
-        close((int)threadIdx.x, kThreads, [&](float x, float unit, auto &&f) { return block_reduce(x, sh.scratch, unit, f); });
-    else if (threadIdx.x < 32)
-        close(lane, 32, [&](float x, float, auto &&f) { return warp_reduce(x, f); });
+    auto in_block = [&](float x, float unit, auto &&f) { return block_reduce(x, sh.scratch, unit, f); };
+    auto in_warp = [&](float x, float, auto &&f) { return warp_reduce(x, f); };
+    if (found > kRanked) {
+        if (found <= NT) close((int)threadIdx.x, NT, std::integral_constant<int, 1>{}, in_block);
+        else if (found <= 2 * NT) close((int)threadIdx.x, NT, std::integral_constant<int, 2>{}, in_block);
+        else close((int)threadIdx.x, NT, std::integral_constant<int, kCandidates / NT>{}, in_block);
+    } else if (threadIdx.x < 32) {
+        if (found <= 32) close(lane, 32, std::integral_constant<int, 1>{}, in_warp);
+        else if (found <= 64) close(lane, 32, std::integral_constant<int, 2>{}, in_warp);
+        else close(lane, 32, std::integral_constant<int, kRanked / 32>{}, in_warp);
+    }
 }
 
 __device__ __forceinline__ float softplus(float d) { return fmaxf(d, 0.f) + log1pf(expf(-fabsf(d))); }
@@ -621,17 +687,19 @@ int afb_top_logits(int64_t rows, int64_t n_moves, int type, const void *logits, 
                                                                               values, moves, log_rest);
                 return;
             }
-            // as few pieces a thread as hold a row wherever it starts
-            auto go = [&](auto p) {
-                top_kernel<T, decltype(p)::value><<<(unsigned)rows, kThreads, 0, s>>>((int)n_moves, x, ld, k, inv_t, values, moves, log_rest);
+            // as few pieces a thread as hold a row wherever it starts; the fewer threads, the more rows at once
+            auto go = [&](auto threads, auto p) {
+                constexpr int NT = decltype(threads)::value;
+                top_kernel<T, NT, decltype(p)::value><<<(unsigned)rows, NT, 0, s>>>((int)n_moves, x, ld, k, inv_t, values, moves, log_rest);
             };
-            const int64_t span = kThreads * Piece<T>::kPer, pieces = (n_moves + Piece<T>::kPer + span - 1) / span;
-            if (pieces <= 1) go(std::integral_constant<int, 1>{});
-            else if (pieces <= 2) go(std::integral_constant<int, 2>{});
-            else if (pieces <= 3) go(std::integral_constant<int, 3>{});
-            else if (pieces <= 5) go(std::integral_constant<int, 5>{});
-            else if (pieces <= 8) go(std::integral_constant<int, 8>{});
-            else go(std::integral_constant<int, 0>{});
+            const int64_t pieces = (n_moves + 2 * Piece<T>::kPer - 2) / Piece<T>::kPer;
+            using Few = std::integral_constant<int, 128>;
+            using Many = std::integral_constant<int, 256>;
+            if (pieces <= 128) go(Few{}, std::integral_constant<int, 1>{});
+            else if (pieces <= 3 * 128) go(Few{}, std::integral_constant<int, 3>{});
+            else if (pieces <= 5 * 128) go(Few{}, std::integral_constant<int, 5>{});
+            else if (pieces <= 9 * 128) go(Few{}, std::integral_constant<int, 9>{});
+            else go(Many{}, std::integral_constant<int, 0>{});
         });
         AFB_LAUNCHED();
     });

@@ -40,7 +40,7 @@ __device__ __forceinline__ int lead_of(const T *row) {
 
 // The piece of a row of n elements that starts at element at (row + at on 16 bytes); what is not of the row is `fill`.
 template <typename T>
-__device__ __forceinline__ Piece<T> load_piece(const T *row, int64_t at, int64_t n, T fill) {
+__device__ __forceinline__ Piece<T> load_piece(const T *row, int at, int n, T fill) {
     Piece<T> v;
     if (at >= 0 && at + Piece<T>::kPer <= n) {
         v.raw = __ldg(reinterpret_cast<const uint4 *>(row + at));

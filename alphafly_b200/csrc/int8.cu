@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int64_t k_di
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const int64_t k = first_of(base, p);
-            mine[p] = k < k_dim ? load_piece(row, k, k_dim, from_float<T>(0.f)) : Piece<T>();
+            mine[p] = k < k_dim ? load_piece(row, (int)k, (int)k_dim, from_float<T>(0.f)) : Piece<T>();
         }
     };
     auto value = [&](int64_t base, int p, int e) {
