@@ -23,8 +23,8 @@ namespace {
 
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 128;                   // of a CTA, but 256 for rows too long for its registers
+constexpr int kWarps = 8;                       // at most
 constexpr int kMaxTop = 256;                    // largest k
 constexpr int kMaxListed = 4096;                // longest list of moves
 constexpr int64_t kMaxMoves = 1 << 20;          // the bitmap of a row's moves fits in shared memory
@@ -75,13 +75,13 @@ __device__ __forceinline__ int block_count(int x, int *scratch) {
 
 // A row's list: moves[l] the l-th listed move, -1 where it does not take part (not valid, out of range, or named before
 // in the list), values[l] its logit.  `bitmap` (n_words) comes back with the moves' bits.
-template <typename T>
+template <int NT, typename T>
 __device__ void read_list(const int64_t *list, const uint8_t *valid, int n_listed, int64_t n_moves, const T *row, unsigned *bitmap,
                           int n_words, int *moves, float *values) {
-    for (int w = threadIdx.x; w < n_words; w += kThreads) bitmap[w] = 0u;
+    for (int w = threadIdx.x; w < n_words; w += NT) bitmap[w] = 0u;
     __syncthreads();
     int again = 0;
-    for (int l = threadIdx.x; l < n_listed; l += kThreads) {
+    for (int l = threadIdx.x; l < n_listed; l += NT) {
         const int64_t m = list[l];
         const bool in = valid[l] && m >= 0 && m < n_moves;
         moves[l] = in ? (int)m : -1;
@@ -91,7 +91,7 @@ __device__ void read_list(const int64_t *list, const uint8_t *valid, int n_liste
         values[l] = to_float(row[m]);
     }
     if (__syncthreads_or(again)) {               // rare: keep the first place of each move, whatever the order above
-        for (int l0 = 0; l0 < n_listed; l0 += kThreads) {
+        for (int l0 = 0; l0 < n_listed; l0 += NT) {
             const int l = n_listed - 1 - l0 - (int)threadIdx.x;             // later places first: theirs are not looked at again
             bool drop = false;
             if (l >= 0 && moves[l] >= 0)
@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(kThreads) top_listed_kernel(int64_t n_moves, c
     const int n_words = (int)((n_moves + 31) / 32);
     int *listed = reinterpret_cast<int *>(dynamic + n_words);
     float *at = reinterpret_cast<float *>(listed + n_listed);
-    read_list(list + i * n_listed, valid + i * n_listed, n_listed, n_moves, row, dynamic, n_words, listed, at);
+    read_list<kThreads>(list + i * n_listed, valid + i * n_listed, n_listed, n_moves, row, dynamic, n_words, listed, at);
     select_top<kThreads>(sh, n_listed, k, inv_t, [&](int e, unsigned &o, int &m) { m = listed[e]; o = m < 0 ? 0u : order_of(at[e]); },
                values + i * k, moves + i * k, log_rest + i);
 }
@@ -486,142 +486,293 @@ struct LossArgs {
     int64_t ld_g;                               // of the gradient
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) loss_kernel(LossArgs a, const T *__restrict__ logits, T *__restrict__ grad) {
-    extern __shared__ unsigned dynamic[];
-    __shared__ float scratch[kWarps];
-    __shared__ int named[kMaxTop];
-    __shared__ float z[kMaxTop], s_at[kMaxTop];
-    const int64_t i = blockIdx.x;
-    const float up = a.upstream ? a.upstream[i * a.upstream_step] : 1.f;
-    if (a.skip_ones && up == 1.f) return;
-    const T *row = logits + i * a.ld;
-    T *g = grad ? grad + i * a.ld_g : nullptr;
-    const float inv_t = 1.f / a.temperature, weight = a.weight ? a.weight[i] : 1.f;
-    const int n_words = (int)((a.n_moves + 31) / 32);
-    unsigned *const bitmap = dynamic;           // the named moves
-    unsigned *const support = dynamic + n_words;                           // the listed moves, their values after them
-    int *const listed = reinterpret_cast<int *>(support + n_words);
-    float *const listed_at = reinterpret_cast<float *>(listed + a.n_listed);
+// The moves that a teacher names in one row, and the log sums over them.
+struct Named {
+    int move[kMaxTop];                          // -1: left out
+    float z[kMaxTop], s[kMaxTop];               // the teacher's logit, the student's
+    float mz, sz, ms, ss;                       // largest z and sum exp((z - mz) / T), the same of s relative to ms (0 for -inf)
+};
 
-    const int n = a.list ? a.n_listed : (int)a.n_moves;
-    if (a.list) read_list(a.list + i * a.n_listed, a.valid + i * a.n_listed, a.n_listed, a.n_moves, row, support, n_words, listed, listed_at);
-    for (int w = threadIdx.x; w < n_words; w += kThreads) bitmap[w] = 0u;
-    for (int c = threadIdx.x; c < a.k; c += kThreads) {
+// Reads row i's named moves and marks them in `marks`, bit move + lead (all threads; the marks are zero, and complete
+// after the return).  keeps(move): whether the student's support has it.
+template <typename T, typename Keeps>
+__device__ void read_named(Named &nm, const LossArgs &a, int64_t i, const T *row, unsigned *marks, int lead, Keeps &&keeps) {
+    int again = 0;
+    for (int c = threadIdx.x; c < a.k; c += blockDim.x) {
         const int64_t m = a.named[i * a.k + c];
         const float t = a.t[i * a.k + c];
-        bool keep = m >= 0 && m < a.n_moves && t != -kInf;
-        if (keep && a.list) keep = (support[m >> 5] >> (m & 31)) & 1u;
-        named[c] = keep ? (int)m : -1;
-        z[c] = t;
+        const bool keep = m >= 0 && m < a.n_moves && t != -kInf && keeps((int)m);
+        nm.move[c] = keep ? (int)m : -1;
+        nm.z[c] = t;
+        nm.s[c] = keep ? to_float(row[m]) : -kInf;
+        if (!keep) continue;
+        const unsigned at = (unsigned)m + lead, bit = 1u << (at & 31);
+        again |= (atomicOr(&marks[at >> 5], bit) & bit) != 0u;
     }
-    __syncthreads();
-    // a move named twice counts at its first place
-    bool twice[(kMaxTop + kThreads - 1) / kThreads];
+    if (__syncthreads_or(again)) {              // rare: a move named twice counts at its first place
+        for (int c0 = 0; c0 < a.k; c0 += blockDim.x) {
+            const int c = a.k - 1 - c0 - (int)threadIdx.x;                  // later places first
+            bool drop = false;
+            if (c >= 0 && nm.move[c] >= 0)
+                for (int d = 0; d < c; ++d) drop |= nm.move[d] == nm.move[c];
+            __syncthreads();
+            if (drop) nm.move[c] = -1;
+            __syncthreads();
+        }
+    }
+}
+
+// One warp: the log sums over the named moves.
+__device__ __forceinline__ void sum_named(Named &nm, int k, float c) {
+    const int lane = threadIdx.x & 31;
+    float mz = -kInf, ms = -kInf, sz = 0.f, ss = 0.f;
+    for (int e = lane; e < k; e += 32)
+        if (nm.move[e] >= 0) {
+            mz = fmaxf(mz, nm.z[e]);
+            ms = fmaxf(ms, nm.s[e]);
+        }
+    mz = warp_reduce(mz, Max());
+    ms = warp_reduce(ms, Max());
+    ms = ms > -kInf ? ms : 0.f;
+    for (int e = lane; e < k; e += 32)
+        if (nm.move[e] >= 0) {
+            sz += exp2_fast((nm.z[e] - mz) * c);
+            ss += exp2_fast((nm.s[e] - ms) * c);
+        }
+    sz = warp_reduce(sz, Sum());
+    ss = warp_reduce(ss, Sum());
+    if (lane == 0) nm.mz = mz, nm.sz = sz, nm.ms = ms, nm.ss = ss;
+}
+
+// What a row's loss and gradient are made of, from the sums over the named moves and over the others (base, sum: the sum
+// of exp((s - base) / T)).  The maxima are subtracted first: the size of the logits does not matter.
+struct Shares {
+    bool some;                                  // a named move, and a move with any probability (a NaN is one)
+    float inv_t, mz, log_sz, ms, log_ss;
+    float odds_p, odds_q, p_rest, log_p_named, log_q_named, log_q_rest;
+    __device__ __forceinline__ Shares(const Named &nm, float temperature, const float *log_rest, float base, float sum) {
+        inv_t = 1.f / temperature;
+        mz = nm.mz;
+        ms = nm.ms;
+        log_sz = logf(nm.sz);
+        log_ss = logf(nm.ss);
+        some = !(nm.sz == 0.f) && !(nm.ss == 0.f && sum == 0.f);
+        odds_q = sum == 0.f ? kInf : nm.ss == 0.f ? -kInf : (ms - base) * inv_t + (log_ss - logf(sum));
+        log_q_rest = -softplus(odds_q);
+        log_q_named = -softplus(-odds_q);
+        odds_p = p_rest = log_p_named = 0.f;
+        if (log_rest && *log_rest != -kInf) {
+            odds_p = mz * inv_t - *log_rest + log_sz;
+            p_rest = expf(-softplus(odds_p));
+            log_p_named = -softplus(-odds_p);
+        }
+    }
+    __device__ __forceinline__ float log_p(float z) const { return (z - mz) * inv_t - log_sz + log_p_named; }
+    __device__ __forceinline__ float log_q(float s) const { return s == -kInf ? -kInf : (s - ms) * inv_t - log_ss + log_q_named; }
+};
+
+// One warp: the row's loss.
+__device__ __forceinline__ void write_loss(const Named &nm, const Shares &sh, const LossArgs &a, int64_t i, float weight) {
+    float part = 0.f;
+    for (int c = threadIdx.x & 31; c < a.k; c += 32)
+        if (nm.move[c] >= 0) {
+            const float lp = sh.log_p(nm.z[c]), p = expf(lp);
+            if (!(p == 0.f)) part += p * (lp - sh.log_q(nm.s[c]));
+        }
+    part = warp_reduce(part, Sum());
+    if ((threadIdx.x & 31) != 0) return;
+    if (!(sh.p_rest == 0.f)) part += sh.p_rest * (softplus(sh.odds_q) - softplus(sh.odds_p));
+    a.loss[i] = sh.some ? part * (a.temperature * a.temperature) * weight : 0.f;
+}
+
+// The gradient at the named moves (all threads).
+template <typename T>
+__device__ __forceinline__ void write_named(const Named &nm, const Shares &sh, int k, float f, T *g) {
+    for (int c = threadIdx.x; c < k; c += blockDim.x)
+        if (nm.move[c] >= 0) g[nm.move[c]] = from_float<T>(sh.some ? f * (expf(sh.log_q(nm.s[c])) - expf(sh.log_p(nm.z[c]))) : 0.f);
+}
+
+// Over a row's listed moves: one CTA per row, the lists and their logits in shared memory.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits, T *__restrict__ grad) {
+    extern __shared__ unsigned dynamic[];
+    __shared__ float scratch[kWarps];
+    __shared__ Named nm;
+    const int n_words = (int)((a.n_moves + 31) / 32), n = a.n_listed;
+    unsigned *const marks = dynamic;            // the named moves, the listed ones, then the list and its logits
+    unsigned *const support = dynamic + n_words;
+    int *const listed = reinterpret_cast<int *>(support + n_words);
+    float *const at = reinterpret_cast<float *>(listed + n);
+    const float c = kLog2e / a.temperature;
+    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+        const float up = a.upstream ? a.upstream[i * a.upstream_step] : 1.f;
+        if (a.skip_ones && up == 1.f) {
+            if (a.upstream_step == 0) return;
+            continue;
+        }
+        const T *row = logits + i * a.ld;
+        const float weight = a.weight ? a.weight[i] : 1.f;
+        T *g = grad ? grad + i * a.ld_g : nullptr;
+        __syncthreads();                        // the row before is done with the shared memory
+        for (int w = threadIdx.x; w < n_words; w += kThreads) marks[w] = 0u;
+        read_list<kThreads>(a.list + i * n, a.valid + i * n, n, a.n_moves, row, support, n_words, listed, at);
+        if (g) {                                // zeros everywhere, the listed moves over them after a barrier
+            const int lead = lead_of(g);
+            const Piece<T> zero;
+            for (int e = (int)threadIdx.x * Piece<T>::kPer - lead; e < a.n_moves; e += kThreads * Piece<T>::kPer)
+                store_piece(g, e, (int)a.n_moves, zero);
+        }
+        read_named(nm, a, i, row, marks, 0, [&](int m) { return ((support[m >> 5] >> (m & 31)) & 1u) != 0u; });
+        if (threadIdx.x < 32) sum_named(nm, a.k, c);
+        auto other = [&](int e) {               // the e-th listed move is in the support and not named
+            const int m = listed[e];
+            return m >= 0 && !((marks[m >> 5] >> (m & 31)) & 1u);
+        };
+        float m = -kInf, sum = 0.f;
+        for (int e = threadIdx.x; e < n; e += kThreads)
+            if (other(e)) m = fmaxf(m, at[e]);
+        m = block_reduce(m, scratch, -kInf, Max());
+        const float base = m > -kInf ? m : 0.f;
+        for (int e = threadIdx.x; e < n; e += kThreads)
+            if (other(e)) sum += exp2_fast((at[e] - base) * c);
+        sum = block_reduce(sum, scratch, 0.f, Sum());
+        const Shares sh(nm, a.temperature, a.log_rest ? a.log_rest + i : nullptr, base, sum);
+        if (a.loss && threadIdx.x < 32) write_loss(nm, sh, a, i, weight);
+        if (!g) continue;
+        const float f = sh.some ? a.temperature * a.scale * weight * up : 0.f;
+        // outside the named moves: the softmax over the rest, times what the student holds there beyond the teacher
+        const float beyond = sum == 0.f ? 0.f : f * (expf(sh.log_q_rest) - sh.p_rest) / sum;
+        for (int e = threadIdx.x; e < n; e += kThreads)
+            if (other(e)) g[listed[e]] = from_float<T>(sh.some ? beyond * exp2_fast((at[e] - base) * c) : 0.f);
+        write_named(nm, sh, a.k, f, g);
+    }
+}
+
+// What a thread of the loss takes of a row at once: one float32, which a warp loads as one line wherever the row starts, so
+// that the order of the sums does not depend on it; a 16-byte piece of a 16-bit type.
+template <typename T>
+struct Part : Piece<T> {
+    static constexpr int kUnits = 1;            // per 16 bytes
+    static __device__ __forceinline__ int lead(const T *row) { return lead_of(row); }
+    __device__ __forceinline__ void load(const T *row, int at, int n) {
+        static_cast<Piece<T> &>(*this) = load_piece(row, at, n, from_float<T>(-kInf));
+    }
+    __device__ __forceinline__ void store(T *row, int at, int n) const { store_piece(row, at, n, *this); }
+};
+template <>
+struct Part<float> {
+    static constexpr int kPer = 1, kUnits = 4;
+    float e[1];
+    static __device__ __forceinline__ int lead(const float *) { return 0; }
+    __device__ __forceinline__ void load(const float *row, int at, int n) { e[0] = at < n ? __ldg(row + at) : -kInf; }
+    __device__ __forceinline__ void store(float *row, int at, int n) const {
+        if (at < n) row[at] = e[0];
+    }
+};
+
+// Over all moves: one CTA of NT threads per row, P times 16 bytes a thread in registers (P = 0: any length, the row is
+// read twice, the second time from cache).  The named moves are taken out of the row (-inf), so that its sum is the rest's;
+// every thread sums relative to its own largest value, and one barrier joins the sums.
+template <typename T, int NT, int P>
+__global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits, T *__restrict__ grad) {
+    constexpr int kPer = Part<T>::kPer, kChunk = (P ? P : 4) * Part<T>::kUnits;
+    extern __shared__ unsigned marks[];         // the named moves, bit move + lead
+    __shared__ float largest[NT / 32], sums[NT / 32];
+    __shared__ Named nm;
+    const int n = (int)a.n_moves, n_words = (n + kPer + 31) / 32, lane = threadIdx.x & 31;
+    const float c = kLog2e / a.temperature;
+    for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
+        const float up = a.upstream ? a.upstream[i * a.upstream_step] : 1.f;
+        if (a.skip_ones && up == 1.f) {
+            if (a.upstream_step == 0) return;
+            continue;
+        }
+        const T *row = logits + i * a.ld;
+        T *g = grad ? grad + i * a.ld_g : nullptr;
+        const int lead = Part<T>::lead(row), first = (int)threadIdx.x * kPer - lead, step = kChunk * NT * kPer;
+        Part<T> mine[kChunk];
+        auto load = [&](int at) {
 #pragma unroll
-    for (int u = 0; u < (kMaxTop + kThreads - 1) / kThreads; ++u) {
-        const int c = u * kThreads + threadIdx.x;
-        twice[u] = false;
-        if (c < a.k && named[c] >= 0)
-            for (int d = 0; d < c; ++d) twice[u] |= named[d] == named[c];
-    }
-    __syncthreads();
+            for (int p = 0; p < kChunk; ++p) mine[p].load(row, at + p * NT * kPer, n);
+        };
+        // the marks of the piece at `at`, whose named moves become -inf
+        auto without_named = [&](Part<T> &v, int at) {
+            const unsigned bits = at < n ? (marks[(at + lead) >> 5] >> ((at + lead) & 31)) & ((1u << kPer) - 1u) : 0u;
+            if (bits)
 #pragma unroll
-    for (int u = 0; u < (kMaxTop + kThreads - 1) / kThreads; ++u) {
-        const int c = u * kThreads + threadIdx.x;
-        if (c >= a.k) break;
-        if (twice[u]) named[c] = -1;
-        s_at[c] = named[c] >= 0 ? to_float(row[named[c]]) : -kInf;
-        if (named[c] >= 0) atomicOr(&bitmap[named[c] >> 5], 1u << (named[c] & 31));
-    }
-    __syncthreads();
-
-    // over the named moves: the teacher's and the student's log sums
-    float mz = -kInf, ms = -kInf;
-    int some = 0;
-    for (int c = threadIdx.x; c < a.k; c += kThreads)
-        if (named[c] >= 0) {
-            some = 1;
-            mz = fmaxf(mz, z[c]);
-            ms = fmaxf(ms, s_at[c]);
-        }
-    some = __syncthreads_or(some);
-    mz = block_reduce(mz, scratch, -kInf, Max());
-    ms = block_reduce(ms, scratch, -kInf, Max());
-    const float base_s = ms > -kInf ? ms : 0.f;
-    float sz = 0.f, ss = 0.f;
-    for (int c = threadIdx.x; c < a.k; c += kThreads)
-        if (named[c] >= 0) {
-            sz += expf((z[c] - mz) * inv_t);
-            ss += expf((s_at[c] - base_s) * inv_t);
-        }
-    sz = block_reduce(sz, scratch, 0.f, Sum());
-    ss = block_reduce(ss, scratch, 0.f, Sum());
-    const float log_sz = logf(sz), log_ss = logf(ss);
-
-    // over the other moves of the support
-    auto other = [&](int e, float &s) {
-        const int m = a.list ? listed[e] : e;
-        if (m < 0) return false;
-        s = a.list ? listed_at[e] : to_float(row[e]);
-        return !((bitmap[m >> 5] >> (m & 31)) & 1u);
-    };
-    float m = -kInf;
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-        float s;
-        if (other(e, s)) m = fmaxf(m, s);
-    }
-    m = block_reduce(m, scratch, -kInf, Max());
-    const float base = m > -kInf ? m : 0.f;
-    float sum = 0.f;
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-        float s;
-        if (other(e, s)) sum += expf((s - base) * inv_t);
-    }
-    sum = block_reduce(sum, scratch, 0.f, Sum());
-    // no move with any probability at all (a NaN is one, and a maximum passes it over)
-    if (ss == 0.f && sum == 0.f) some = 0;
-
-    // log odds and log shares of the named moves against the rest: the student's, and the teacher's where it has a rest.
-    // The maxima are subtracted first: the size of the logits does not matter.
-    const float log_sum = logf(sum);
-    const float odds_q = sum == 0.f ? kInf : ss == 0.f ? -kInf : (base_s - base) * inv_t + (log_ss - log_sum);
-    const float log_q_rest = -softplus(odds_q), log_q_named = -softplus(-odds_q);
-    float odds_p = 0.f, p_rest = 0.f, log_p_named = 0.f;
-    if (a.log_rest && a.log_rest[i] != -kInf) {
-        odds_p = mz * inv_t - a.log_rest[i] + log_sz;
-        p_rest = expf(-softplus(odds_p));
-        log_p_named = -softplus(-odds_p);
-    }
-    auto log_p = [&](int c) { return (z[c] - mz) * inv_t - log_sz + log_p_named; };
-    auto log_q = [&](int c) { return s_at[c] == -kInf ? -kInf : (s_at[c] - base_s) * inv_t - log_ss + log_q_named; };
-    if (a.loss) {
-        float part = 0.f;
-        for (int c = threadIdx.x; c < a.k; c += kThreads)
-            if (named[c] >= 0) {
-                const float lp = log_p(c), p = expf(lp);
-                if (!(p == 0.f)) part += p * (lp - log_q(c));
-            }
-        part = block_reduce(part, scratch, 0.f, Sum());
-        if (threadIdx.x == 0) {
-            if (!(p_rest == 0.f)) part += p_rest * (softplus(odds_q) - softplus(odds_p));
-            a.loss[i] = some ? part * (a.temperature * a.temperature) * weight : 0.f;
-        }
-    }
-    if (!g) return;
-    const float f = some ? a.temperature * a.scale * weight * up : 0.f;
-    // outside the named moves: the softmax over the rest, times what the student holds there beyond the teacher
-    const float beyond = sum == 0.f ? 0.f : f * (expf(log_q_rest) - p_rest) / sum;
-    if (a.list) {
-        for (int64_t e = threadIdx.x; e < a.n_moves; e += kThreads) g[e] = from_float<T>(0.f);
+                for (int e = 0; e < kPer; ++e)
+                    if ((bits >> e) & 1u) v.e[e] = from_float<T>(-kInf);
+            return bits;
+        };
+        if (P) load(first);
+        __syncthreads();                        // the row before is done with the shared memory
+        for (int w = threadIdx.x; w < n_words; w += NT) marks[w] = 0u;
         __syncthreads();
+        read_named(nm, a, i, row, marks, lead, [](int) { return true; });
+        if (threadIdx.x < 32) sum_named(nm, a.k, c);
+
+        float m = -kInf, sum = 0.f;             // sum relative to m, or to 0 while m is -inf
+        for (int at = first; at < n; at += step) {
+            if (!P) load(at);
+            float top = m;
+#pragma unroll
+            for (int p = 0; p < kChunk; ++p) {
+                without_named(mine[p], at + p * NT * kPer);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) top = fmaxf(top, to_float(mine[p].e[e]));
+            }
+            if (m > -kInf) sum *= exp2_fast((m - top) * c);
+            m = top;
+            const float from = m > -kInf ? m : 0.f;
+#pragma unroll
+            for (int p = 0; p < kChunk; ++p)
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) sum += exp2_fast((to_float(mine[p].e[e]) - from) * c);
+            if (P) break;
+        }
+        const float warp_m = warp_reduce(m, Max());
+        sum *= m > -kInf ? exp2_fast((m - warp_m) * c) : 1.f;               // 0 or NaN without a largest value
+        sum = warp_reduce(sum, Sum());
+        if (lane == 0) largest[threadIdx.x >> 5] = warp_m, sums[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        m = -kInf;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) m = fmaxf(m, largest[w]);
+        const float base = m > -kInf ? m : 0.f;
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) sum += sums[w] * (largest[w] > -kInf ? exp2_fast((largest[w] - base) * c) : 1.f);
+        const Shares sh(nm, a.temperature, a.log_rest ? a.log_rest + i : nullptr, base, sum);
+        const float weight = a.weight ? a.weight[i] : 1.f;
+        if (a.loss && threadIdx.x < 32) write_loss(nm, sh, a, i, weight);
+        if (!g) continue;
+        const float f = sh.some ? a.temperature * a.scale * weight * up : 0.f;
+        // outside the named moves: the softmax over the rest, times what the student holds there beyond the teacher
+        const float beyond = sum == 0.f || !sh.some ? 0.f : f * (expf(sh.log_q_rest) - sh.p_rest) / sum;
+        const bool aligned = Part<T>::lead(g) == lead;
+        for (int at0 = first; at0 < n; at0 += step) {
+            if (!P) load(at0);
+#pragma unroll
+            for (int p = 0; p < kChunk; ++p) {
+                const int at = at0 + p * NT * kPer;
+                if (at >= n) break;
+                const unsigned bits = without_named(mine[p], at);
+                Part<T> out;
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    out.e[e] = from_float<T>(sh.some ? beyond * exp2_fast((to_float(mine[p].e[e]) - base) * c) : 0.f);
+                if (bits == 0u && aligned) {
+                    out.store(g, at, n);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e)
+                        if (at + e >= 0 && at + e < n && !((bits >> e) & 1u)) g[at + e] = out.e[e];
+                }
+            }
+            if (P) break;
+        }
+        write_named(nm, sh, a.k, f, g);
     }
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-        float s;
-        if (other(e, s)) g[a.list ? listed[e] : e] = from_float<T>(some ? beyond * expf((s - base) * inv_t) : 0.f);
-    }
-    for (int c = threadIdx.x; c < a.k; c += kThreads)
-        if (named[c] >= 0) g[named[c]] = from_float<T>(some ? f * (expf(log_q(c)) - expf(log_p(c))) : 0.f);
 }
 
 // out = scale * sum of the losses, in one fixed order.
@@ -639,6 +790,19 @@ __global__ void __launch_bounds__(1024) sum_kernel(int64_t rows, const float *__
         for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
         if (threadIdx.x == 0) *out = (float)(x * scale);
     }
+}
+
+// Threads of a CTA and 16-byte pieces a thread for rows of n elements: as few as hold a row wherever it starts (few
+// threads: many rows at once); 256 and 0, no row in registers, beyond 4,605 float32 or 9,209 16-bit elements.
+template <typename T, typename F>
+void by_row_length(int64_t n, F &&f) {
+    const int64_t pieces = (n + 2 * Piece<T>::kPer - 2) / Piece<T>::kPer;
+    using Few = std::integral_constant<int, kThreads>;
+    if (pieces <= kThreads) f(Few{}, std::integral_constant<int, 1>{});
+    else if (pieces <= 3 * kThreads) f(Few{}, std::integral_constant<int, 3>{});
+    else if (pieces <= 5 * kThreads) f(Few{}, std::integral_constant<int, 5>{});
+    else if (pieces <= 9 * kThreads) f(Few{}, std::integral_constant<int, 9>{});
+    else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
 }
 
 template <typename K>
@@ -687,19 +851,10 @@ int afb_top_logits(int64_t rows, int64_t n_moves, int type, const void *logits, 
                                                                               values, moves, log_rest);
                 return;
             }
-            // as few pieces a thread as hold a row wherever it starts; the fewer threads, the more rows at once
-            auto go = [&](auto threads, auto p) {
+            by_row_length<T>(n_moves, [&](auto threads, auto p) {
                 constexpr int NT = decltype(threads)::value;
                 top_kernel<T, NT, decltype(p)::value><<<(unsigned)rows, NT, 0, s>>>((int)n_moves, x, ld, k, inv_t, values, moves, log_rest);
-            };
-            const int64_t pieces = (n_moves + 2 * Piece<T>::kPer - 2) / Piece<T>::kPer;
-            using Few = std::integral_constant<int, 128>;
-            using Many = std::integral_constant<int, 256>;
-            if (pieces <= 128) go(Few{}, std::integral_constant<int, 1>{});
-            else if (pieces <= 3 * 128) go(Few{}, std::integral_constant<int, 3>{});
-            else if (pieces <= 5 * 128) go(Few{}, std::integral_constant<int, 5>{});
-            else if (pieces <= 9 * 128) go(Few{}, std::integral_constant<int, 9>{});
-            else go(Many{}, std::integral_constant<int, 0>{});
+            });
         });
         AFB_LAUNCHED();
     });
@@ -724,12 +879,25 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
         }
         const LossArgs a{n_moves, ld, values, moves, log_rest, k, temperature, legal, valid, (int)n_listed, weight, scale, upstream,
                          upstream_step, skip_ones, row_loss, ld_grad};
-        const size_t words = (size_t)((n_moves + 31) / 32) * 4;
-        const size_t shared = legal ? 2 * words + (size_t)n_listed * 8 : words;
+        const cudaStream_t s = as_stream(stream);
         with_type(type, [&](auto e) {
             using T = decltype(e);
-            allow_shared(loss_kernel<T>, shared);
-            loss_kernel<T><<<(unsigned)rows, kThreads, shared, as_stream(stream)>>>(a, static_cast<const T *>(logits), static_cast<T *>(grad));
+            const T *x = static_cast<const T *>(logits);
+            T *g = static_cast<T *>(grad);
+            // a call that may have nothing to do is not worth a CTA per row
+            const unsigned grid = (unsigned)(skip_ones ? std::min<int64_t>(rows, 148 * 8) : rows);
+            if (legal) {
+                const size_t shared = (size_t)((n_moves + 31) / 32) * 8 + (size_t)n_listed * 8;
+                allow_shared(loss_listed_kernel<T>, shared);
+                loss_listed_kernel<T><<<grid, kThreads, shared, s>>>(a, rows, x, g);
+                return;
+            }
+            const size_t shared = (size_t)((n_moves + Piece<T>::kPer + 31) / 32) * 4;
+            by_row_length<T>(n_moves, [&](auto threads, auto p) {
+                constexpr int NT = decltype(threads)::value;
+                allow_shared(loss_kernel<T, NT, decltype(p)::value>, shared);
+                loss_kernel<T, NT, decltype(p)::value><<<grid, NT, shared, s>>>(a, rows, x, g);
+            });
         });
         AFB_LAUNCHED();
         if (loss) {

@@ -51,6 +51,18 @@ __device__ __forceinline__ Piece<T> load_piece(const T *row, int at, int n, T fi
     return v;
 }
 
+// Stores a piece over the elements from `at` on, those of them that are of the row (row + at on 16 bytes).
+template <typename T>
+__device__ __forceinline__ void store_piece(T *row, int at, int n, const Piece<T> &v) {
+    if (at >= 0 && at + Piece<T>::kPer <= n) {
+        *reinterpret_cast<uint4 *>(row + at) = v.raw;
+    } else {
+#pragma unroll
+        for (int e = 0; e < Piece<T>::kPer; ++e)
+            if (at + e >= 0 && at + e < n) row[at + e] = v.e[e];
+    }
+}
+
 inline bool known_type(int t) { return t == AFB_T_F32 || t == AFB_T_F16 || t == AFB_T_BF16; }
 inline size_t type_size(int t) { return t == AFB_T_F32 ? 4 : 2; }
 
