@@ -493,10 +493,10 @@ struct Named {
     float mz, sz, ms, ss;                       // largest z and sum exp((z - mz) / T), the same of s relative to ms (0 for -inf)
 };
 
-// Reads row i's named moves and marks them in `marks`, bit move + lead (all threads; the marks are zero, and complete
-// after the return).  keeps(move): whether the student's support has it.
-template <typename T, typename Keeps>
-__device__ void read_named(Named &nm, const LossArgs &a, int64_t i, const T *row, unsigned *marks, int lead, Keeps &&keeps) {
+// Reads row i's named moves and marks them (all threads; the marks are complete after the return).  keeps(move): whether
+// the student's support has it; mark(move): sets its mark, whether it was set already.
+template <typename T, typename Keeps, typename Mark>
+__device__ void read_named(Named &nm, const LossArgs &a, int64_t i, const T *row, Keeps &&keeps, Mark &&mark) {
     int again = 0;
     for (int c = threadIdx.x; c < a.k; c += blockDim.x) {
         const int64_t m = a.named[i * a.k + c];
@@ -505,9 +505,7 @@ __device__ void read_named(Named &nm, const LossArgs &a, int64_t i, const T *row
         nm.move[c] = keep ? (int)m : -1;
         nm.z[c] = t;
         nm.s[c] = keep ? to_float(row[m]) : -kInf;
-        if (!keep) continue;
-        const unsigned at = (unsigned)m + lead, bit = 1u << (at & 31);
-        again |= (atomicOr(&marks[at >> 5], bit) & bit) != 0u;
+        if (keep) again |= mark((int)m);
     }
     if (__syncthreads_or(again)) {              // rare: a move named twice counts at its first place
         for (int c0 = 0; c0 < a.k; c0 += blockDim.x) {
@@ -585,11 +583,31 @@ __device__ __forceinline__ void write_loss(const Named &nm, const Shares &sh, co
     a.loss[i] = sh.some ? part * (a.temperature * a.temperature) * weight : 0.f;
 }
 
-// The gradient at the named moves (all threads).
+// One warp: the gradient at the named moves.
 template <typename T>
 __device__ __forceinline__ void write_named(const Named &nm, const Shares &sh, int k, float f, T *g) {
-    for (int c = threadIdx.x; c < k; c += blockDim.x)
+    for (int c = threadIdx.x & 31; c < k; c += 32)
         if (nm.move[c] >= 0) g[nm.move[c]] = from_float<T>(sh.some ? f * (expf(sh.log_q(nm.s[c])) - expf(sh.log_p(nm.z[c]))) : 0.f);
+}
+
+// The gradient outside the named moves: the softmax over them, times what the student holds there beyond the teacher.
+struct OtherPart {
+    float base, beyond;
+    __device__ __forceinline__ float of(float s, float c) const { return beyond == 0.f ? 0.f : beyond * exp2_fast((s - base) * c); }
+};
+
+// One warp: a row's loss and the gradient at its named moves, and what the gradient at the others is made of.
+template <typename T>
+__device__ __forceinline__ void close_row(const Named &nm, OtherPart &part, const LossArgs &a, int64_t i, float base, float sum,
+                                          float weight, float up, T *g) {
+    const Shares sh(nm, a.temperature, a.log_rest ? a.log_rest + i : nullptr, base, sum);
+    const float f = a.temperature * a.scale * weight * up;
+    if ((threadIdx.x & 31) == 0) {
+        part.base = base;
+        part.beyond = sum == 0.f || !sh.some ? 0.f : f * (expf(sh.log_q_rest) - sh.p_rest) / sum;
+    }
+    if (a.loss) write_loss(nm, sh, a, i, weight);
+    if (g) write_named(nm, sh, a.k, f, g);
 }
 
 // Over a row's listed moves: one CTA per row, the lists and their logits in shared memory.
@@ -598,6 +616,7 @@ __global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64
     extern __shared__ unsigned dynamic[];
     __shared__ float scratch[kWarps];
     __shared__ Named nm;
+    __shared__ OtherPart part;
     const int n_words = (int)((a.n_moves + 31) / 32), n = a.n_listed;
     unsigned *const marks = dynamic;            // the named moves, the listed ones, then the list and its logits
     unsigned *const support = dynamic + n_words;
@@ -622,7 +641,8 @@ __global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64
             for (int e = (int)threadIdx.x * Piece<T>::kPer - lead; e < a.n_moves; e += kThreads * Piece<T>::kPer)
                 store_piece(g, e, (int)a.n_moves, zero);
         }
-        read_named(nm, a, i, row, marks, 0, [&](int m) { return ((support[m >> 5] >> (m & 31)) & 1u) != 0u; });
+        read_named(nm, a, i, row, [&](int m) { return ((support[m >> 5] >> (m & 31)) & 1u) != 0u; },
+                   [&](int m) { return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u); });
         if (threadIdx.x < 32) sum_named(nm, a.k, c);
         auto other = [&](int e) {               // the e-th listed move is in the support and not named
             const int m = listed[e];
@@ -636,15 +656,11 @@ __global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64
         for (int e = threadIdx.x; e < n; e += kThreads)
             if (other(e)) sum += exp2_fast((at[e] - base) * c);
         sum = block_reduce(sum, scratch, 0.f, Sum());
-        const Shares sh(nm, a.temperature, a.log_rest ? a.log_rest + i : nullptr, base, sum);
-        if (a.loss && threadIdx.x < 32) write_loss(nm, sh, a, i, weight);
+        if (threadIdx.x < 32) close_row(nm, part, a, i, base, sum, weight, up, g);
         if (!g) continue;
-        const float f = sh.some ? a.temperature * a.scale * weight * up : 0.f;
-        // outside the named moves: the softmax over the rest, times what the student holds there beyond the teacher
-        const float beyond = sum == 0.f ? 0.f : f * (expf(sh.log_q_rest) - sh.p_rest) / sum;
+        __syncthreads();
         for (int e = threadIdx.x; e < n; e += kThreads)
-            if (other(e)) g[listed[e]] = from_float<T>(sh.some ? beyond * exp2_fast((at[e] - base) * c) : 0.f);
-        write_named(nm, sh, a.k, f, g);
+            if (other(e)) g[listed[e]] = from_float<T>(part.of(at[e], c));
     }
 }
 
@@ -673,13 +689,24 @@ struct Part<float> {
 // Over all moves: one CTA of NT threads per row, P times 16 bytes a thread in registers (P = 0: any length, the row is
 // read twice, the second time from cache).  The named moves are taken out of the row (-inf), so that its sum is the rest's;
 // every thread sums relative to its own largest value, and one barrier joins the sums.
+// Words of marks a thread: a bit for each of its kChunk kPer places, or (0) for each 32 of a row of n moves.
+template <int kPer, int NT, int kChunk>
+__host__ __device__ constexpr int mark_words(int n) {
+    return kChunk ? (kChunk * kPer + 31) / 32 : ((n + kPer - 1) / kPer / NT + 1) * kPer / 32 + 1;
+}
+
 template <typename T, int NT, int P>
-__global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits, T *__restrict__ grad) {
-    constexpr int kPer = Part<T>::kPer, kChunk = (P ? P : 4) * Part<T>::kUnits;
-    extern __shared__ unsigned marks[];         // the named moves, bit move + lead
+__global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) loss_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits,
+                                                                     T *__restrict__ grad) {
+    // without registers for the row, 32 moves a thread at a time
+    constexpr int kPer = Part<T>::kPer, kChunk = P ? P * Part<T>::kUnits : 32 / kPer;
+    constexpr bool kKeep = P > 0 && sizeof(T) == 4;                      // the exponentials stay in the row's registers
+    extern __shared__ unsigned marks[];         // of the named moves: bits of a thread's moves in its order, words NT apart
     __shared__ float largest[NT / 32], sums[NT / 32];
     __shared__ Named nm;
-    const int n = (int)a.n_moves, n_words = (n + kPer + 31) / 32, lane = threadIdx.x & 31;
+    __shared__ OtherPart part;
+    const int n = (int)a.n_moves, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n_words = mark_words<kPer, NT, P ? kChunk : 0>(n);
     const float c = kLog2e / a.temperature;
     for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
         const float up = a.upstream ? a.upstream[i * a.upstream_step] : 1.f;
@@ -695,83 +722,95 @@ __global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, cons
 #pragma unroll
             for (int p = 0; p < kChunk; ++p) mine[p].load(row, at + p * NT * kPer, n);
         };
-        // the marks of the piece at `at`, whose named moves become -inf
-        auto without_named = [&](Part<T> &v, int at) {
-            const unsigned bits = at < n ? (marks[(at + lead) >> 5] >> ((at + lead) & 31)) & ((1u << kPer) - 1u) : 0u;
-            if (bits)
-#pragma unroll
-                for (int e = 0; e < kPer; ++e)
-                    if ((bits >> e) & 1u) v.e[e] = from_float<T>(-kInf);
-            return bits;
-        };
         if (P) load(first);
         __syncthreads();                        // the row before is done with the shared memory
-        for (int w = threadIdx.x; w < n_words; w += NT) marks[w] = 0u;
+        for (int w = 0; w < n_words; ++w) marks[w * NT + threadIdx.x] = 0u;
         __syncthreads();
-        read_named(nm, a, i, row, marks, lead, [](int) { return true; });
-        if (threadIdx.x < 32) sum_named(nm, a.k, c);
-
+        read_named(nm, a, i, row, [](int) { return true; },
+                   [&](int m) {
+                       const int q = m + lead, t = q / kPer % NT, bit = q / kPer / NT * kPer + q % kPer;
+                       return (int)((atomicOr(&marks[(bit >> 5) * NT + t], 1u << (bit & 31)) >> (bit & 31)) & 1u);
+                   });
+        // the named moves of the chunk whose first bit is bit0 become -inf
+        auto drop_named = [&](int bit0) {
+#pragma unroll
+            for (int w = 0; w < (kChunk * kPer + 31) / 32; ++w) {
+                const unsigned word = marks[(bit0 / 32 + w) * NT + threadIdx.x];
+                if (word)
+#pragma unroll
+                    for (int b = 0; b < 32; ++b) {
+                        const int p = (w * 32 + b) / kPer;
+                        if (p < kChunk && ((word >> b) & 1u)) mine[p < kChunk ? p : 0].e[b % kPer] = from_float<T>(-kInf);
+                    }
+            }
+        };
         float m = -kInf, sum = 0.f;             // sum relative to m, or to 0 while m is -inf
-        for (int at = first; at < n; at += step) {
+        for (int at = first, bit0 = 0; at < n; at += step, bit0 += 32) {
             if (!P) load(at);
+            drop_named(bit0);
             float top = m;
 #pragma unroll
-            for (int p = 0; p < kChunk; ++p) {
-                without_named(mine[p], at + p * NT * kPer);
+            for (int p = 0; p < kChunk; ++p)
 #pragma unroll
                 for (int e = 0; e < kPer; ++e) top = fmaxf(top, to_float(mine[p].e[e]));
-            }
             if (m > -kInf) sum *= exp2_fast((m - top) * c);
             m = top;
             const float from = m > -kInf ? m : 0.f;
 #pragma unroll
             for (int p = 0; p < kChunk; ++p)
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) sum += exp2_fast((to_float(mine[p].e[e]) - from) * c);
+                for (int e = 0; e < kPer; ++e) {
+                    const float x = exp2_fast((to_float(mine[p].e[e]) - from) * c);
+                    if constexpr (kKeep) mine[p].e[e] = x;
+                    sum += x;
+                }
             if (P) break;
         }
         const float warp_m = warp_reduce(m, Max());
         sum *= m > -kInf ? exp2_fast((m - warp_m) * c) : 1.f;               // 0 or NaN without a largest value
         sum = warp_reduce(sum, Sum());
-        if (lane == 0) largest[threadIdx.x >> 5] = warp_m, sums[threadIdx.x >> 5] = sum;
+        if (lane == 0) largest[warp] = warp_m, sums[warp] = sum;
+        if (warp == 0) sum_named(nm, a.k, c);
         __syncthreads();
-        m = -kInf;
+        if (warp == 0) {
+            float all = -kInf, total = 0.f;
 #pragma unroll
-        for (int w = 0; w < NT / 32; ++w) m = fmaxf(m, largest[w]);
-        const float base = m > -kInf ? m : 0.f;
-        sum = 0.f;
+            for (int w = 0; w < NT / 32; ++w) all = fmaxf(all, largest[w]);
+            const float base = all > -kInf ? all : 0.f;
 #pragma unroll
-        for (int w = 0; w < NT / 32; ++w) sum += sums[w] * (largest[w] > -kInf ? exp2_fast((largest[w] - base) * c) : 1.f);
-        const Shares sh(nm, a.temperature, a.log_rest ? a.log_rest + i : nullptr, base, sum);
-        const float weight = a.weight ? a.weight[i] : 1.f;
-        if (a.loss && threadIdx.x < 32) write_loss(nm, sh, a, i, weight);
+            for (int w = 0; w < NT / 32; ++w) total += sums[w] * (largest[w] > -kInf ? exp2_fast((largest[w] - base) * c) : 1.f);
+            close_row(nm, part, a, i, base, total, a.weight ? a.weight[i] : 1.f, up, g);
+        }
         if (!g) continue;
-        const float f = sh.some ? a.temperature * a.scale * weight * up : 0.f;
-        // outside the named moves: the softmax over the rest, times what the student holds there beyond the teacher
-        const float beyond = sum == 0.f || !sh.some ? 0.f : f * (expf(sh.log_q_rest) - sh.p_rest) / sum;
+        __syncthreads();
+        // the named moves are written by the warp above
+        const float keep = m > -kInf ? part.of(m, c) : part.beyond * 0.f;    // of this thread's exponentials
         const bool aligned = Part<T>::lead(g) == lead;
-        for (int at0 = first; at0 < n; at0 += step) {
+        for (int at0 = first, bit0 = 0; at0 < n; at0 += step, bit0 += 32) {
             if (!P) load(at0);
+            unsigned word = 0u;
 #pragma unroll
             for (int p = 0; p < kChunk; ++p) {
-                const int at = at0 + p * NT * kPer;
+                const int at = at0 + p * NT * kPer, bit = p * kPer;
+                if (bit % 32 == 0) word = marks[(bit0 + bit) / 32 * NT + threadIdx.x];
                 if (at >= n) break;
-                const unsigned bits = without_named(mine[p], at);
+                const unsigned named = (word >> (bit % 32)) & ((1u << kPer) - 1u);
                 Part<T> out;
 #pragma unroll
-                for (int e = 0; e < kPer; ++e)
-                    out.e[e] = from_float<T>(sh.some ? beyond * exp2_fast((to_float(mine[p].e[e]) - base) * c) : 0.f);
-                if (bits == 0u && aligned) {
+                for (int e = 0; e < kPer; ++e) {
+                    const float x = to_float(mine[p].e[e]);
+                    out.e[e] = from_float<T>(!kKeep ? part.of(x, c) : keep == 0.f ? 0.f : keep * x);
+                }
+                if (named == 0u && aligned) {
                     out.store(g, at, n);
                 } else {
 #pragma unroll
                     for (int e = 0; e < kPer; ++e)
-                        if (at + e >= 0 && at + e < n && !((bits >> e) & 1u)) g[at + e] = out.e[e];
+                        if (at + e >= 0 && at + e < n && !((named >> e) & 1u)) g[at + e] = out.e[e];
                 }
             }
             if (P) break;
         }
-        write_named(nm, sh, a.k, f, g);
     }
 }
 
@@ -892,9 +931,9 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
                 loss_listed_kernel<T><<<grid, kThreads, shared, s>>>(a, rows, x, g);
                 return;
             }
-            const size_t shared = (size_t)((n_moves + Piece<T>::kPer + 31) / 32) * 4;
             by_row_length<T>(n_moves, [&](auto threads, auto p) {
-                constexpr int NT = decltype(threads)::value;
+                constexpr int NT = decltype(threads)::value, kChunk = decltype(p)::value * Part<T>::kUnits;
+                const size_t shared = (size_t)mark_words<Part<T>::kPer, NT, kChunk>((int)n_moves) * NT * 4;
                 allow_shared(loss_kernel<T, NT, decltype(p)::value>, shared);
                 loss_kernel<T, NT, decltype(p)::value><<<grid, NT, shared, s>>>(a, rows, x, g);
             });
