@@ -22,9 +22,10 @@ namespace afb {
 namespace {
 
 constexpr float kInf = __builtin_huge_valf();
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 128;                   // of a CTA, but 256 for rows too long for its registers
-constexpr int kWarps = 8;                       // at most
+constexpr int kWarps = 16;                      // at most
+constexpr int kLongThreads = 256;               // for rows that a CTA does not hold
 constexpr int kMaxTop = 256;                    // largest k
 constexpr int kMaxListed = 4096;                // longest list of moves
 constexpr int64_t kMaxMoves = 1 << 20;          // the bitmap of a row's moves fits in shared memory
@@ -486,25 +487,48 @@ struct LossArgs {
     int64_t ld_g;                               // of the gradient
 };
 
-// The moves that a teacher names in one row, and the log sums over them.
+// The moves that a teacher names in one row, and what is known of them before the row's other moves are summed, all in
+// shared memory.
+struct NamedSums {
+    float p_rest, log_p_rest;                   // of any other move (0 and -inf without a rest)
+    float ms, log_ss;                           // largest s (0 for -inf), log sum exp((s - ms) / T)
+    int some;                                   // a move is named
+};
 struct Named {
-    int move[kMaxTop];                          // -1: left out
-    float z[kMaxTop], s[kMaxTop];               // the teacher's logit, the student's
-    float mz, sz, ms, ss;                       // largest z and sum exp((z - mz) / T), the same of s relative to ms (0 for -inf)
+    int *move;                                  // -1: left out
+    float *z, *s, *p;                           // the teacher's logit, then log p; the student's logit; p
+    NamedSums *sums;
+    __host__ __device__ static constexpr size_t bytes(int k) { return (size_t)k * 16; }
+    __device__ __forceinline__ Named(unsigned char *at, int k, NamedSums *sums) : move(reinterpret_cast<int *>(at)), sums(sums) {
+        z = reinterpret_cast<float *>(at) + k;
+        s = z + k;
+        p = s + k;
+    }
+};
+
+// A thread's first named move, asked for before anything else of the row.
+struct FirstNamed {
+    int64_t move = -1;
+    float t = 0.f;
+    __device__ __forceinline__ FirstNamed(const LossArgs &a, int64_t i) {
+        if ((int)threadIdx.x < a.k) move = a.named[i * a.k + threadIdx.x], t = a.t[i * a.k + threadIdx.x];
+    }
 };
 
 // Reads row i's named moves and marks them (all threads; the marks are complete after the return).  keeps(move): whether
-// the student's support has it; mark(move): sets its mark, whether it was set already.
-template <typename T, typename Keeps, typename Mark>
-__device__ void read_named(Named &nm, const LossArgs &a, int64_t i, const T *row, Keeps &&keeps, Mark &&mark) {
+// the student's support has it; value(move): the student's logit; mark(move): sets its mark, whether it was set already.
+template <typename T, typename Keeps, typename Value, typename Mark>
+__device__ __forceinline__ void read_named(const Named &nm, const LossArgs &a, int64_t i, const T *row, const FirstNamed &first,
+                                           Keeps &&keeps, Value &&value, Mark &&mark) {
     int again = 0;
     for (int c = threadIdx.x; c < a.k; c += blockDim.x) {
-        const int64_t m = a.named[i * a.k + c];
-        const float t = a.t[i * a.k + c];
+        const bool fetched = c == (int)threadIdx.x;
+        const int64_t m = fetched ? first.move : a.named[i * a.k + c];
+        const float t = fetched ? first.t : a.t[i * a.k + c];
         const bool keep = m >= 0 && m < a.n_moves && t != -kInf && keeps((int)m);
         nm.move[c] = keep ? (int)m : -1;
         nm.z[c] = t;
-        nm.s[c] = keep ? to_float(row[m]) : -kInf;
+        nm.s[c] = keep ? value((int)m) : -kInf;
         if (keep) again |= mark((int)m);
     }
     if (__syncthreads_or(again)) {              // rare: a move named twice counts at its first place
@@ -517,97 +541,93 @@ __device__ void read_named(Named &nm, const LossArgs &a, int64_t i, const T *row
             if (drop) nm.move[c] = -1;
             __syncthreads();
         }
+        for (int c = threadIdx.x; c < a.k; c += blockDim.x)
+            if (nm.move[c] >= 0) nm.s[c] = to_float(row[nm.move[c]]);       // whichever of them had read it
+        __syncthreads();
     }
 }
 
-// One warp: the log sums over the named moves.
-__device__ __forceinline__ void sum_named(Named &nm, int k, float c) {
+// One warp: the teacher's distribution.  The shares of the named moves and of the rest follow from their log odds.
+__device__ __forceinline__ void teach(const Named &nm, const LossArgs &a, int64_t i, float c, float inv_t) {
     const int lane = threadIdx.x & 31;
-    float mz = -kInf, ms = -kInf, sz = 0.f, ss = 0.f;
-    for (int e = lane; e < k; e += 32)
-        if (nm.move[e] >= 0) {
-            mz = fmaxf(mz, nm.z[e]);
-            ms = fmaxf(ms, nm.s[e]);
-        }
+    float mz = -kInf, sz = 0.f;
+    int some = 0;
+    for (int e = lane; e < a.k; e += 32)
+        if (nm.move[e] >= 0) mz = fmaxf(mz, nm.z[e]), some = 1;
     mz = warp_reduce(mz, Max());
+    for (int e = lane; e < a.k; e += 32)
+        if (nm.move[e] >= 0) sz += exp2_fast((nm.z[e] - mz) * c);
+    sz = warp_reduce(sz, Sum());
+    const float log_sz = logf(sz), log_rest = a.log_rest ? a.log_rest[i] : -kInf;
+    const float odds = mz * inv_t - log_rest + log_sz;                   // inf without a rest
+    const float log_p_rest = -softplus(odds), log_p_named = -softplus(-odds);
+    for (int e = lane; e < a.k; e += 32)
+        if (nm.move[e] >= 0) {
+            nm.z[e] = (nm.z[e] - mz) * inv_t - log_sz + log_p_named;
+            nm.p[e] = expf(nm.z[e]);
+        }
+    some = __any_sync(0xffffffffu, some);
+    if (lane == 0) nm.sums->p_rest = expf(log_p_rest), nm.sums->log_p_rest = log_p_rest, nm.sums->some = some;
+}
+
+// One warp: the student's log sum over the named moves.
+__device__ __forceinline__ void sum_named(const Named &nm, int k, float c) {
+    const int lane = threadIdx.x & 31;
+    float ms = -kInf, ss = 0.f;
+    for (int e = lane; e < k; e += 32)
+        if (nm.move[e] >= 0) ms = fmaxf(ms, nm.s[e]);
     ms = warp_reduce(ms, Max());
     ms = ms > -kInf ? ms : 0.f;
     for (int e = lane; e < k; e += 32)
-        if (nm.move[e] >= 0) {
-            sz += exp2_fast((nm.z[e] - mz) * c);
-            ss += exp2_fast((nm.s[e] - ms) * c);
-        }
-    sz = warp_reduce(sz, Sum());
+        if (nm.move[e] >= 0) ss += exp2_fast((nm.s[e] - ms) * c);
     ss = warp_reduce(ss, Sum());
-    if (lane == 0) nm.mz = mz, nm.sz = sz, nm.ms = ms, nm.ss = ss;
+    if (lane == 0) nm.sums->ms = ms, nm.sums->log_ss = logf(ss);
 }
 
-// What a row's loss and gradient are made of, from the sums over the named moves and over the others (base, sum: the sum
-// of exp((s - base) / T)).  The maxima are subtracted first: the size of the logits does not matter.
-struct Shares {
-    bool some;                                  // a named move, and a move with any probability (a NaN is one)
-    float inv_t, mz, log_sz, ms, log_ss;
-    float odds_p, odds_q, p_rest, log_p_named, log_q_named, log_q_rest;
-    __device__ __forceinline__ Shares(const Named &nm, float temperature, const float *log_rest, float base, float sum) {
-        inv_t = 1.f / temperature;
-        mz = nm.mz;
-        ms = nm.ms;
-        log_sz = logf(nm.sz);
-        log_ss = logf(nm.ss);
-        some = !(nm.sz == 0.f) && !(nm.ss == 0.f && sum == 0.f);
-        odds_q = sum == 0.f ? kInf : nm.ss == 0.f ? -kInf : (ms - base) * inv_t + (log_ss - logf(sum));
-        log_q_rest = -softplus(odds_q);
-        log_q_named = -softplus(-odds_q);
-        odds_p = p_rest = log_p_named = 0.f;
-        if (log_rest && *log_rest != -kInf) {
-            odds_p = mz * inv_t - *log_rest + log_sz;
-            p_rest = expf(-softplus(odds_p));
-            log_p_named = -softplus(-odds_p);
-        }
-    }
-    __device__ __forceinline__ float log_p(float z) const { return (z - mz) * inv_t - log_sz + log_p_named; }
-    __device__ __forceinline__ float log_q(float s) const { return s == -kInf ? -kInf : (s - ms) * inv_t - log_ss + log_q_named; }
-};
+// The student's log odds of the named moves against the others, whose terms sum to `sum` relative to exp(reference); gap:
+// by how much ms / T exceeds the reference.  The maxima are subtracted first: the size of the logits does not matter.
+__device__ __forceinline__ float odds_of(const Named &nm, float gap, float sum) {
+    return sum == 0.f ? (nm.sums->log_ss == -kInf ? 0.f : kInf) : gap + (nm.sums->log_ss - logf(sum));
+}
+// Whether a row has something to learn: a named move, and a move with any probability (a NaN is one).
+__device__ __forceinline__ bool alive(const Named &nm, float sum) { return nm.sums->some && !(nm.sums->log_ss == -kInf && sum == 0.f); }
 
-// One warp: the row's loss.
-__device__ __forceinline__ void write_loss(const Named &nm, const Shares &sh, const LossArgs &a, int64_t i, float weight) {
+// The gradient at a move that is not named over its term of `sum`: the softmax over those moves, times what the student
+// holds there beyond the teacher (1 / (1 + exp(odds)) - p_rest).
+__device__ __forceinline__ float beyond_of(const Named &nm, float odds, float sum, float f) {
+    return sum == 0.f || !alive(nm, sum) ? 0.f : f * (1.f / (1.f + expf(odds)) - nm.sums->p_rest) / sum;
+}
+// The gradient at a move from its term: 0 where nothing is to be learnt, whatever the term.
+__device__ __forceinline__ float times(float beyond, float term) { return beyond == 0.f ? 0.f : beyond * term; }
+
+// log q of the e-th named move.
+__device__ __forceinline__ float log_q_of(const Named &nm, int e, float log_q_named, float inv_t) {
+    const float s = nm.s[e];
+    return s == -kInf ? -kInf : (s - nm.sums->ms) * inv_t + log_q_named;
+}
+__device__ __forceinline__ float log_q_named_of(const Named &nm, float odds) { return -softplus(-odds) - nm.sums->log_ss; }
+
+// One warp: a row's loss.
+__device__ __forceinline__ void write_loss(const Named &nm, const LossArgs &a, int64_t i, float odds, float sum, float inv_t, float weight) {
+    const float log_q_named = log_q_named_of(nm, odds);
     float part = 0.f;
-    for (int c = threadIdx.x & 31; c < a.k; c += 32)
-        if (nm.move[c] >= 0) {
-            const float lp = sh.log_p(nm.z[c]), p = expf(lp);
-            if (!(p == 0.f)) part += p * (lp - sh.log_q(nm.s[c]));
+    for (int e = threadIdx.x & 31; e < a.k; e += 32)
+        if (nm.move[e] >= 0) {
+            const float p = nm.p[e];
+            if (!(p == 0.f)) part += p * (nm.z[e] - log_q_of(nm, e, log_q_named, inv_t));
         }
     part = warp_reduce(part, Sum());
-    if ((threadIdx.x & 31) != 0) return;
-    if (!(sh.p_rest == 0.f)) part += sh.p_rest * (softplus(sh.odds_q) - softplus(sh.odds_p));
-    a.loss[i] = sh.some ? part * (a.temperature * a.temperature) * weight : 0.f;
+    if (!(nm.sums->p_rest == 0.f)) part += nm.sums->p_rest * (nm.sums->log_p_rest + softplus(odds));
+    if ((threadIdx.x & 31) == 0) a.loss[i] = alive(nm, sum) ? part * (a.temperature * a.temperature) * weight : 0.f;
 }
 
-// One warp: the gradient at the named moves.
+// The gradient at the named moves (all threads, over what stands there).
 template <typename T>
-__device__ __forceinline__ void write_named(const Named &nm, const Shares &sh, int k, float f, T *g) {
-    for (int c = threadIdx.x & 31; c < k; c += 32)
-        if (nm.move[c] >= 0) g[nm.move[c]] = from_float<T>(sh.some ? f * (expf(sh.log_q(nm.s[c])) - expf(sh.log_p(nm.z[c]))) : 0.f);
-}
-
-// The gradient outside the named moves: the softmax over them, times what the student holds there beyond the teacher.
-struct OtherPart {
-    float base, beyond;
-    __device__ __forceinline__ float of(float s, float c) const { return beyond == 0.f ? 0.f : beyond * exp2_fast((s - base) * c); }
-};
-
-// One warp: a row's loss and the gradient at its named moves, and what the gradient at the others is made of.
-template <typename T>
-__device__ __forceinline__ void close_row(const Named &nm, OtherPart &part, const LossArgs &a, int64_t i, float base, float sum,
-                                          float weight, float up, T *g) {
-    const Shares sh(nm, a.temperature, a.log_rest ? a.log_rest + i : nullptr, base, sum);
-    const float f = a.temperature * a.scale * weight * up;
-    if ((threadIdx.x & 31) == 0) {
-        part.base = base;
-        part.beyond = sum == 0.f || !sh.some ? 0.f : f * (expf(sh.log_q_rest) - sh.p_rest) / sum;
-    }
-    if (a.loss) write_loss(nm, sh, a, i, weight);
-    if (g) write_named(nm, sh, a.k, f, g);
+__device__ __forceinline__ void write_named(const Named &nm, int k, float odds, float sum, float inv_t, float f, T *g) {
+    const bool some = alive(nm, sum);
+    for (int e = threadIdx.x; e < k; e += blockDim.x)
+        if (nm.move[e] >= 0)
+            g[nm.move[e]] = from_float<T>(some ? f * (expf(log_q_of(nm, e, log_q_named_of(nm, odds), inv_t)) - nm.p[e]) : 0.f);
 }
 
 // Over a row's listed moves: one CTA per row, the lists and their logits in shared memory.
@@ -615,14 +635,14 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits, T *__restrict__ grad) {
     extern __shared__ unsigned dynamic[];
     __shared__ float scratch[kWarps];
-    __shared__ Named nm;
-    __shared__ OtherPart part;
+    __shared__ NamedSums named_sums;
     const int n_words = (int)((a.n_moves + 31) / 32), n = a.n_listed;
-    unsigned *const marks = dynamic;            // the named moves, the listed ones, then the list and its logits
+    unsigned *const marks = dynamic;            // the named moves, the listed ones, then the list, its logits, the named
     unsigned *const support = dynamic + n_words;
     int *const listed = reinterpret_cast<int *>(support + n_words);
     float *const at = reinterpret_cast<float *>(listed + n);
-    const float c = kLog2e / a.temperature;
+    const Named nm(reinterpret_cast<unsigned char *>(at + n), a.k, &named_sums);
+    const float inv_t = 1.f / a.temperature, c = kLog2e * inv_t;
     for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
         const float up = a.upstream ? a.upstream[i * a.upstream_step] : 1.f;
         if (a.skip_ones && up == 1.f) {
@@ -630,6 +650,7 @@ __global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64
             continue;
         }
         const T *row = logits + i * a.ld;
+        const FirstNamed first_named(a, i);
         const float weight = a.weight ? a.weight[i] : 1.f;
         T *g = grad ? grad + i * a.ld_g : nullptr;
         __syncthreads();                        // the row before is done with the shared memory
@@ -641,9 +662,11 @@ __global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64
             for (int e = (int)threadIdx.x * Piece<T>::kPer - lead; e < a.n_moves; e += kThreads * Piece<T>::kPer)
                 store_piece(g, e, (int)a.n_moves, zero);
         }
-        read_named(nm, a, i, row, [&](int m) { return ((support[m >> 5] >> (m & 31)) & 1u) != 0u; },
-                   [&](int m) { return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u); });
-        if (threadIdx.x < 32) sum_named(nm, a.k, c);
+        read_named(nm, a, i, row, first_named, [&](int m) { return ((support[m >> 5] >> (m & 31)) & 1u) != 0u; },
+                   [&](int m) { return to_float(row[m]); }, [&](int m) { return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u); });
+        const int role = (int)(threadIdx.x >> 5);
+        if (role == 0) sum_named(nm, a.k, c);
+        else if (role == 1) teach(nm, a, i, c, inv_t);
         auto other = [&](int e) {               // the e-th listed move is in the support and not named
             const int m = listed[e];
             return m >= 0 && !((marks[m >> 5] >> (m & 31)) & 1u);
@@ -656,58 +679,190 @@ __global__ void __launch_bounds__(kThreads) loss_listed_kernel(LossArgs a, int64
         for (int e = threadIdx.x; e < n; e += kThreads)
             if (other(e)) sum += exp2_fast((at[e] - base) * c);
         sum = block_reduce(sum, scratch, 0.f, Sum());
-        if (threadIdx.x < 32) close_row(nm, part, a, i, base, sum, weight, up, g);
+        const float f = a.temperature * a.scale * weight * up, odds = odds_of(nm, (nm.sums->ms - base) * inv_t, sum);
+        if (a.loss && role == 0) write_loss(nm, a, i, odds, sum, inv_t, weight);
         if (!g) continue;
-        __syncthreads();
+        write_named(nm, a.k, odds, sum, inv_t, f, g);
+        const float beyond = beyond_of(nm, odds, sum, f);
         for (int e = threadIdx.x; e < n; e += kThreads)
-            if (other(e)) g[listed[e]] = from_float<T>(part.of(at[e], c));
+            if (other(e)) g[listed[e]] = from_float<T>(times(beyond, exp2_fast((at[e] - base) * c)));
     }
 }
 
-// What a thread of the loss takes of a row at once: one float32, which a warp loads as one line wherever the row starts, so
-// that the order of the sums does not depend on it; a 16-byte piece of a 16-bit type.
+// Where a row's elements lie in shared memory: float32 from the start, so that the order of the sums does not depend on
+// where the row starts in memory; 16-bit types as far from 16 bytes as there, so that they move in 16-byte pieces.
 template <typename T>
-struct Part : Piece<T> {
-    static constexpr int kUnits = 1;            // per 16 bytes
-    static __device__ __forceinline__ int lead(const T *row) { return lead_of(row); }
-    __device__ __forceinline__ void load(const T *row, int at, int n) {
-        static_cast<Piece<T> &>(*this) = load_piece(row, at, n, from_float<T>(-kInf));
-    }
-    __device__ __forceinline__ void store(T *row, int at, int n) const { store_piece(row, at, n, *this); }
-};
-template <>
-struct Part<float> {
-    static constexpr int kPer = 1, kUnits = 4;
-    float e[1];
-    static __device__ __forceinline__ int lead(const float *) { return 0; }
-    __device__ __forceinline__ void load(const float *row, int at, int n) { e[0] = at < n ? __ldg(row + at) : -kInf; }
-    __device__ __forceinline__ void store(float *row, int at, int n) const {
-        if (at < n) row[at] = e[0];
-    }
-};
+__device__ __forceinline__ int shift_of(const T *row) { return sizeof(T) == 4 ? 0 : lead_of(row); }
 
-// Over all moves: one CTA of NT threads per row, P times 16 bytes a thread in registers (P = 0: any length, the row is
-// read twice, the second time from cache).  The named moves are taken out of the row (-inf), so that its sum is the rest's;
-// every thread sums relative to its own largest value, and one barrier joins the sums.
-// Words of marks a thread: a bit for each of its kChunk kPer places, or (0) for each 32 of a row of n moves.
-template <int kPer, int NT, int kChunk>
-__host__ __device__ constexpr int mark_words(int n) {
-    return kChunk ? (kChunk * kPer + 31) / 32 : ((n + kPer - 1) / kPer / NT + 1) * kPer / 32 + 1;
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void *shared, const void *global) {
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(shared);
+    if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(global) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(dst), "l"(global) : "memory");
+}
+template <int kPending>
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;\n" ::"n"(kPending) : "memory"); }
+
+// Starts the copy of a row of n elements to held[shift_of(row)] on; what is not of the row in its 16-byte pieces is -inf.
+template <int NT, typename T>
+__device__ __forceinline__ void fetch_row(T *held, const T *row, int n) {
+    constexpr int kPer = Piece<T>::kPer;
+    const int shift = shift_of(row), pieces = (shift + n + kPer - 1) / kPer;
+    const bool whole = lead_of(row) == shift;    // pieces of the row start on 16 bytes
+    for (int p = threadIdx.x; p < pieces; p += NT) {
+        const int at = p * kPer - shift;
+        T *const dst = held + p * kPer;
+        if (whole && at >= 0 && at + kPer <= n) {
+            copy_async<16>(dst, row + at);
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            if (at + e < 0 || at + e >= n) dst[e] = from_float<T>(-kInf);
+            else if (sizeof(T) == 4) copy_async<4>(dst + e, row + at + e);
+            else dst[e] = row[at + e];
+        }
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
 }
 
-template <typename T, int NT, int P>
-__global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) loss_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits,
-                                                                     T *__restrict__ grad) {
-    // without registers for the row, 32 moves a thread at a time
-    constexpr int kPer = Part<T>::kPer, kChunk = P ? P * Part<T>::kUnits : 32 / kPer;
-    constexpr bool kKeep = P > 0 && sizeof(T) == 4;                      // the exponentials stay in the row's registers
-    extern __shared__ unsigned marks[];         // of the named moves: bits of a thread's moves in its order, words NT apart
-    __shared__ float largest[NT / 32], sums[NT / 32];
-    __shared__ Named nm;
-    __shared__ OtherPart part;
+// Over all moves, rows held in shared memory, NT threads a row.  The CTAs stay: with kAhead a CTA's next row is on its way
+// (into a second buffer) while it works on one, so that only shared memory is waited for.  The named moves are taken out
+// of the row (-inf), so that its sum is the rest's.  The terms are relative to the student's best named move: no maximum
+// is taken, one barrier joins the sums.  A sum outside kSmall .. kLarge (a rest 69 T from that move, no such move, NaN,
+// values whose product with 1 / T overflows) is taken again, after subtracting the largest.
+constexpr float kSmall = 1e-30f, kLarge = 1e30f;
+
+template <typename T, int NT, bool kAhead>
+__global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, int held_bytes, const T *__restrict__ logits,
+                                                  T *__restrict__ grad) {
+    constexpr int kPer = Piece<T>::kPer;
+    constexpr bool kKeep = sizeof(T) == 4;      // the terms replace the logits in shared memory
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ float scratch[kWarps];
+    __shared__ NamedSums named_sums;
+    // the rows' buffers, the named moves, their marks
+    const Named nm(raw + (kAhead ? 2 : 1) * held_bytes, a.k, &named_sums);
+    unsigned *const marks = reinterpret_cast<unsigned *>(nm.p + a.k);
     const int n = (int)a.n_moves, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int n_words = mark_words<kPer, NT, P ? kChunk : 0>(n);
-    const float c = kLog2e / a.temperature;
+    const float inv_t = 1.f / a.temperature, c = kLog2e * inv_t;
+    auto held_of = [&](int turn) { return reinterpret_cast<T *>(raw + (kAhead ? turn * held_bytes : 0)); };
+    // the first row of this CTA from i on that is not left as it is
+    auto next = [&](int64_t i) {
+        if (a.skip_ones)
+            while (i < rows && a.upstream[i * a.upstream_step] == 1.f) i = a.upstream_step ? i + gridDim.x : rows;
+        return i;
+    };
+    int64_t i = next(blockIdx.x);
+    if (i >= rows) return;
+    for (int w = threadIdx.x; w < (n + 31) / 32; w += NT) marks[w] = 0u;
+    FirstNamed first_named(a, i);
+    fetch_row<NT>(held_of(0), logits + i * a.ld, n);
+    for (int turn = 0; i < rows; turn ^= 1) {
+        const T *row = logits + i * a.ld;
+        T *g = grad ? grad + i * a.ld_g : nullptr;
+        T *const held = held_of(turn);
+        const int shift = shift_of(row), pieces = (shift + n + kPer - 1) / kPer;
+        const int64_t after = next(i + gridDim.x);
+        if (kAhead && after < rows) {
+            fetch_row<NT>(held_of(turn ^ 1), logits + after * a.ld, n);
+            copies_done<1>();
+        } else {
+            copies_done<0>();
+        }
+        __syncthreads();
+        read_named(nm, a, i, row, first_named, [](int) { return true; }, [&](int m) { return to_float(held[shift + m]); },
+                   [&](int m) {
+                       held[shift + m] = from_float<T>(-kInf);
+                       return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u);
+                   });
+        if (after < rows) first_named = FirstNamed(a, after);
+        float ref = -kInf;                      // every warp for itself
+        for (int e = lane; e < a.k; e += 32)
+            if (nm.move[e] >= 0) ref = fmaxf(ref, nm.s[e]);
+        ref = warp_reduce(ref, Max()) * c;      // a term is 2^(s c - ref): one rounding of the exponent
+        float sum = 0.f;
+#pragma unroll 4
+        for (int p = threadIdx.x; p < pieces; p += NT) {
+            Piece<T> v;
+            v.raw = *reinterpret_cast<const uint4 *>(held + p * kPer);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) {
+                const float x = exp2_fast(fmaf(to_float(v.e[e]), c, -ref));
+                if constexpr (kKeep) v.e[e] = x;
+                sum += x;
+            }
+            if constexpr (kKeep) *reinterpret_cast<uint4 *>(held + p * kPer) = v.raw;
+        }
+        if (warp == 0) sum_named(nm, a.k, c);
+        else if (warp == 1) teach(nm, a, i, c, inv_t);
+        sum = warp_reduce(sum, Sum());
+        if (lane == 0) scratch[warp] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < NT / 32; ++w) sum += scratch[w];
+        const float weight = a.weight ? a.weight[i] : 1.f, f = a.temperature * a.scale * weight * (a.upstream ? a.upstream[i * a.upstream_step] : 1.f);
+        const bool again = !(sum > kSmall && sum < kLarge);
+        float gap = fmaf(nm.sums->ms, c, -ref) * kLn2, base = -kInf;
+        if (again) {
+            __syncthreads();
+            for (int m = threadIdx.x; m < n; m += NT) {
+                held[shift + m] = (marks[m >> 5] >> (m & 31)) & 1u ? from_float<T>(-kInf) : row[m];
+                base = fmaxf(base, to_float(held[shift + m]));
+            }
+            base = block_reduce(base, scratch, -kInf, Max());
+            base = base > -kInf ? base : 0.f;
+            sum = 0.f;
+            for (int m = threadIdx.x; m < n; m += NT) {
+                const float x = exp2_fast((to_float(held[shift + m]) - base) * c);
+                if constexpr (kKeep) held[shift + m] = x;
+                sum += x;
+            }
+            sum = block_reduce(sum, scratch, 0.f, Sum());
+            gap = (nm.sums->ms - base) * inv_t;
+        }
+        const float odds = odds_of(nm, gap, sum);
+        if (a.loss && warp == 0) write_loss(nm, a, i, odds, sum, inv_t, weight);
+        if (g) {
+            const float beyond = beyond_of(nm, odds, sum, f);
+            auto gradient = [&](T v) {
+                const float s = to_float(v);
+                if (again) return from_float<T>(times(beyond, kKeep ? s : exp2_fast((s - base) * c)));
+                return from_float<T>(beyond * (kKeep ? s : exp2_fast(fmaf(s, c, -ref))));
+            };
+            if (lead_of(g) == shift) {
+#pragma unroll 4
+                for (int p = threadIdx.x; p < pieces; p += NT) {
+                    Piece<T> v;
+                    v.raw = *reinterpret_cast<const uint4 *>(held + p * kPer);
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) v.e[e] = gradient(v.e[e]);
+                    store_piece(g, p * kPer - shift, n, v);
+                }
+            } else {
+                for (int m = threadIdx.x; m < n; m += NT) g[m] = gradient(held[shift + m]);
+            }
+            __syncthreads();
+            write_named(nm, a.k, odds, sum, inv_t, f, g);
+        }
+        for (int e = threadIdx.x; e < a.k; e += NT)
+            if (nm.move[e] >= 0) marks[nm.move[e] >> 5] = 0u;
+        if (!kAhead && after < rows) fetch_row<NT>(held_of(0), logits + after * a.ld, n);
+        i = after;
+    }
+}
+
+// Rows too long for shared memory: read twice, the second time from cache.  As above, but for the marks: no row is held.
+template <typename T>
+__global__ void __launch_bounds__(kLongThreads) loss_long_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits, T *__restrict__ grad) {
+    constexpr int kPer = Piece<T>::kPer, kChunk = 4;
+    extern __shared__ unsigned marks[];
+    __shared__ float scratch[kWarps];
+    __shared__ NamedSums named_sums;
+    const int n = (int)a.n_moves, words = (n + 31) / 32, warp = threadIdx.x >> 5;
+    const Named nm(reinterpret_cast<unsigned char *>(marks + words), a.k, &named_sums);
+    const float inv_t = 1.f / a.temperature, c = kLog2e * inv_t;
     for (int64_t i = blockIdx.x; i < rows; i += gridDim.x) {
         const float up = a.upstream ? a.upstream[i * a.upstream_step] : 1.f;
         if (a.skip_ones && up == 1.f) {
@@ -716,101 +871,78 @@ __global__ void __launch_bounds__(NT, NT == 128 ? 8 : 4) loss_kernel(LossArgs a,
         }
         const T *row = logits + i * a.ld;
         T *g = grad ? grad + i * a.ld_g : nullptr;
-        const int lead = Part<T>::lead(row), first = (int)threadIdx.x * kPer - lead, step = kChunk * NT * kPer;
-        Part<T> mine[kChunk];
-        auto load = [&](int at) {
-#pragma unroll
-            for (int p = 0; p < kChunk; ++p) mine[p].load(row, at + p * NT * kPer, n);
-        };
-        if (P) load(first);
+        const int shift = shift_of(row), first = (int)threadIdx.x * kPer - shift, step = kLongThreads * kPer;
+        const bool whole = lead_of(row) == shift;
+        const FirstNamed first_named(a, i);
         __syncthreads();                        // the row before is done with the shared memory
-        for (int w = 0; w < n_words; ++w) marks[w * NT + threadIdx.x] = 0u;
+        for (int w = threadIdx.x; w < words; w += kLongThreads) marks[w] = 0u;
         __syncthreads();
-        read_named(nm, a, i, row, [](int) { return true; },
-                   [&](int m) {
-                       const int q = m + lead, t = q / kPer % NT, bit = q / kPer / NT * kPer + q % kPer;
-                       return (int)((atomicOr(&marks[(bit >> 5) * NT + t], 1u << (bit & 31)) >> (bit & 31)) & 1u);
-                   });
-        // the named moves of the chunk whose first bit is bit0 become -inf
-        auto drop_named = [&](int bit0) {
+        read_named(nm, a, i, row, first_named, [](int) { return true; }, [&](int m) { return to_float(row[m]); },
+                   [&](int m) { return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u); });
+        if (warp == 0) sum_named(nm, a.k, c);
+        else if (warp == 1) teach(nm, a, i, c, inv_t);
+        // f(piece, its first element) of this thread's pieces, the named moves -inf
+        auto each = [&](auto &&f) {
+            for (int at0 = first; at0 < n; at0 += kChunk * step) {
+                Piece<T> v[kChunk];
 #pragma unroll
-            for (int w = 0; w < (kChunk * kPer + 31) / 32; ++w) {
-                const unsigned word = marks[(bit0 / 32 + w) * NT + threadIdx.x];
-                if (word)
+                for (int p = 0; p < kChunk; ++p) {
+                    const int at = at0 + p * step;
+                    if (whole) {
+                        v[p] = load_piece(row, at, n, from_float<T>(-kInf));
+                    } else {
 #pragma unroll
-                    for (int b = 0; b < 32; ++b) {
-                        const int p = (w * 32 + b) / kPer;
-                        if (p < kChunk && ((word >> b) & 1u)) mine[p < kChunk ? p : 0].e[b % kPer] = from_float<T>(-kInf);
+                        for (int e = 0; e < kPer; ++e) v[p].e[e] = at + e < n ? row[at + e] : from_float<T>(-kInf);
                     }
+                }
+#pragma unroll
+                for (int p = 0; p < kChunk; ++p) {
+                    const int at = at0 + p * step;
+                    if (at >= n) break;
+                    // the marks of elements at .. at + kPer - 1, which may lie in two words
+                    const int from = max(at, 0);
+                    const unsigned low = marks[from >> 5], high = marks[min((from >> 5) + 1, words - 1)];
+                    unsigned bits = __funnelshift_r(low, high, from & 31) << (from - at);
+                    if (bits & ((1u << kPer) - 1u))
+#pragma unroll
+                        for (int e = 0; e < kPer; ++e)
+                            if ((bits >> e) & 1u) v[p].e[e] = from_float<T>(-kInf);
+                    f(v[p], at);
+                }
             }
         };
-        float m = -kInf, sum = 0.f;             // sum relative to m, or to 0 while m is -inf
-        for (int at = first, bit0 = 0; at < n; at += step, bit0 += 32) {
-            if (!P) load(at);
-            drop_named(bit0);
-            float top = m;
+        float m = -kInf, sum = 0.f;
+        each([&](const Piece<T> &v, int) {
 #pragma unroll
-            for (int p = 0; p < kChunk; ++p)
+            for (int e = 0; e < kPer; ++e) m = fmaxf(m, to_float(v.e[e]));
+        });
+        m = block_reduce(m, scratch, -kInf, Max());
+        const float base = m > -kInf ? m : 0.f;
+        each([&](const Piece<T> &v, int) {
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) top = fmaxf(top, to_float(mine[p].e[e]));
-            if (m > -kInf) sum *= exp2_fast((m - top) * c);
-            m = top;
-            const float from = m > -kInf ? m : 0.f;
-#pragma unroll
-            for (int p = 0; p < kChunk; ++p)
-#pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const float x = exp2_fast((to_float(mine[p].e[e]) - from) * c);
-                    if constexpr (kKeep) mine[p].e[e] = x;
-                    sum += x;
-                }
-            if (P) break;
-        }
-        const float warp_m = warp_reduce(m, Max());
-        sum *= m > -kInf ? exp2_fast((m - warp_m) * c) : 1.f;               // 0 or NaN without a largest value
-        sum = warp_reduce(sum, Sum());
-        if (lane == 0) largest[warp] = warp_m, sums[warp] = sum;
-        if (warp == 0) sum_named(nm, a.k, c);
-        __syncthreads();
-        if (warp == 0) {
-            float all = -kInf, total = 0.f;
-#pragma unroll
-            for (int w = 0; w < NT / 32; ++w) all = fmaxf(all, largest[w]);
-            const float base = all > -kInf ? all : 0.f;
-#pragma unroll
-            for (int w = 0; w < NT / 32; ++w) total += sums[w] * (largest[w] > -kInf ? exp2_fast((largest[w] - base) * c) : 1.f);
-            close_row(nm, part, a, i, base, total, a.weight ? a.weight[i] : 1.f, up, g);
-        }
+            for (int e = 0; e < kPer; ++e) sum += exp2_fast((to_float(v.e[e]) - base) * c);
+        });
+        sum = block_reduce(sum, scratch, 0.f, Sum());
+        const float weight = a.weight ? a.weight[i] : 1.f, f = a.temperature * a.scale * weight * up;
+        const float odds = odds_of(nm, (nm.sums->ms - base) * inv_t, sum);
+        if (a.loss && warp == 0) write_loss(nm, a, i, odds, sum, inv_t, weight);
         if (!g) continue;
-        __syncthreads();
-        // the named moves are written by the warp above
-        const float keep = m > -kInf ? part.of(m, c) : part.beyond * 0.f;    // of this thread's exponentials
-        const bool aligned = Part<T>::lead(g) == lead;
-        for (int at0 = first, bit0 = 0; at0 < n; at0 += step, bit0 += 32) {
-            if (!P) load(at0);
-            unsigned word = 0u;
+        const float beyond = beyond_of(nm, odds, sum, f);
+        const bool aligned = lead_of(g) == shift;
+        each([&](const Piece<T> &v, int at) {
+            Piece<T> out;
 #pragma unroll
-            for (int p = 0; p < kChunk; ++p) {
-                const int at = at0 + p * NT * kPer, bit = p * kPer;
-                if (bit % 32 == 0) word = marks[(bit0 + bit) / 32 * NT + threadIdx.x];
-                if (at >= n) break;
-                const unsigned named = (word >> (bit % 32)) & ((1u << kPer) - 1u);
-                Part<T> out;
+            for (int e = 0; e < kPer; ++e) out.e[e] = from_float<T>(times(beyond, exp2_fast((to_float(v.e[e]) - base) * c)));
+            if (aligned) {
+                store_piece(g, at, n, out);
+            } else {
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const float x = to_float(mine[p].e[e]);
-                    out.e[e] = from_float<T>(!kKeep ? part.of(x, c) : keep == 0.f ? 0.f : keep * x);
-                }
-                if (named == 0u && aligned) {
-                    out.store(g, at, n);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e)
-                        if (at + e >= 0 && at + e < n && !((named >> e) & 1u)) g[at + e] = out.e[e];
-                }
+                for (int e = 0; e < kPer; ++e)
+                    if (at + e >= 0 && at + e < n) g[at + e] = out.e[e];
             }
-            if (P) break;
-        }
+        });
+        __syncthreads();
+        write_named(nm, a.k, odds, sum, inv_t, f, g);
     }
 }
 
@@ -923,20 +1055,33 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
             using T = decltype(e);
             const T *x = static_cast<const T *>(logits);
             T *g = static_cast<T *>(grad);
-            // a call that may have nothing to do is not worth a CTA per row
-            const unsigned grid = (unsigned)(skip_ones ? std::min<int64_t>(rows, 148 * 8) : rows);
             if (legal) {
-                const size_t shared = (size_t)((n_moves + 31) / 32) * 8 + (size_t)n_listed * 8;
+                const size_t shared = (size_t)((n_moves + 31) / 32) * 8 + (size_t)n_listed * 8 + Named::bytes(k);
                 allow_shared(loss_listed_kernel<T>, shared);
+                // a call that may have nothing to do is not worth a CTA per row
+                const unsigned grid = (unsigned)(skip_ones ? std::min<int64_t>(rows, 148 * 8) : rows);
                 loss_listed_kernel<T><<<grid, kThreads, shared, s>>>(a, rows, x, g);
                 return;
             }
-            by_row_length<T>(n_moves, [&](auto threads, auto p) {
-                constexpr int NT = decltype(threads)::value, kChunk = decltype(p)::value * Part<T>::kUnits;
-                const size_t shared = (size_t)mark_words<Part<T>::kPer, NT, kChunk>((int)n_moves) * NT * 4;
-                allow_shared(loss_kernel<T, NT, decltype(p)::value>, shared);
-                loss_kernel<T, NT, decltype(p)::value><<<grid, NT, shared, s>>>(a, rows, x, g);
-            });
+            const size_t held = ((size_t)(n_moves + 2 * Piece<T>::kPer) * sizeof(T) + 15) / 16 * 16;
+            const size_t more = Named::bytes(k) + (size_t)((n_moves + 31) / 32) * 4;
+            auto go = [&](auto threads, auto ahead) {
+                constexpr int NT = decltype(threads)::value;
+                auto kernel = loss_kernel<T, NT, decltype(ahead)::value>;
+                const size_t shared = (decltype(ahead)::value ? 2 : 1) * held + more;
+                allow_shared(kernel, shared);
+                // as many CTAs as the device holds: 228 KB of shared memory an SM, of which a CTA takes 1.2 KB besides
+                const int64_t ctas = std::min<int64_t>(2048 / NT, 228 * 1024 / (shared + 1280));
+                kernel<<<(unsigned)std::min<int64_t>(rows, 148 * ctas), NT, shared, s>>>(a, rows, (int)held, x, g);
+            };
+            if (held <= 20 * 1024) go(std::integral_constant<int, 128>{}, std::true_type{});
+            else if (held <= 36 * 1024) go(std::integral_constant<int, 256>{}, std::true_type{});
+            else if (held + more <= 112 * 1024) go(std::integral_constant<int, 256>{}, std::false_type{});
+            else {
+                const size_t shared = more;
+                allow_shared(loss_long_kernel<T>, shared);
+                loss_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 8), kLongThreads, shared, s>>>(a, rows, x, g);
+            }
         });
         AFB_LAUNCHED();
         if (loss) {
