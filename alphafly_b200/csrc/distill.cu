@@ -976,9 +976,16 @@ void by_row_length(int64_t n, F &&f) {
     else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
 }
 
-template <typename K>
-void allow_shared(K kernel, size_t bytes) {
-    if (bytes > 32 * 1024) AFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// Lets the kernel take that much dynamic shared memory on the current device; asked for once per size that is needed.
+template <auto kKernel>
+void allow_shared(size_t bytes) {
+    static size_t allowed[64] = {0};
+    if (bytes <= 32 * 1024) return;
+    int dev = 0;
+    AFB_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && allowed[dev] >= bytes) return;
+    AFB_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) allowed[dev] = bytes;
 }
 
 void check_rows(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k, float temperature,
@@ -1017,7 +1024,7 @@ int afb_top_logits(int64_t rows, int64_t n_moves, int type, const void *logits, 
             const T *x = static_cast<const T *>(logits);
             if (legal) {
                 const size_t shared = (size_t)((n_moves + 31) / 32) * 4 + (size_t)n_listed * 8;
-                allow_shared(top_listed_kernel<T>, shared);
+                allow_shared<top_listed_kernel<T>>(shared);
                 top_listed_kernel<T><<<(unsigned)rows, kThreads, shared, s>>>(n_moves, x, ld, k, inv_t, legal, valid, (int)n_listed,
                                                                               values, moves, log_rest);
                 return;
@@ -1057,7 +1064,7 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
             T *g = static_cast<T *>(grad);
             if (legal) {
                 const size_t shared = (size_t)((n_moves + 31) / 32) * 8 + (size_t)n_listed * 8 + Named::bytes(k);
-                allow_shared(loss_listed_kernel<T>, shared);
+                allow_shared<loss_listed_kernel<T>>(shared);
                 // a call that may have nothing to do is not worth a CTA per row
                 const unsigned grid = (unsigned)(skip_ones ? std::min<int64_t>(rows, 148 * 8) : rows);
                 loss_listed_kernel<T><<<grid, kThreads, shared, s>>>(a, rows, x, g);
@@ -1067,9 +1074,9 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
             const size_t more = Named::bytes(k) + (size_t)((n_moves + 31) / 32) * 4;
             auto go = [&](auto threads, auto ahead) {
                 constexpr int NT = decltype(threads)::value;
-                auto kernel = loss_kernel<T, NT, decltype(ahead)::value>;
+                constexpr auto kernel = loss_kernel<T, NT, decltype(ahead)::value>;
                 const size_t shared = (decltype(ahead)::value ? 2 : 1) * held + more;
-                allow_shared(kernel, shared);
+                allow_shared<kernel>(shared);
                 // as many CTAs as the device holds: 228 KB of shared memory an SM, of which a CTA takes 1.2 KB besides
                 const int64_t ctas = std::min<int64_t>(2048 / NT, 228 * 1024 / (shared + 1280));
                 kernel<<<(unsigned)std::min<int64_t>(rows, 148 * ctas), NT, shared, s>>>(a, rows, (int)held, x, g);
@@ -1079,7 +1086,7 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
             else if (held + more <= 112 * 1024) go(std::integral_constant<int, 256>{}, std::false_type{});
             else {
                 const size_t shared = more;
-                allow_shared(loss_long_kernel<T>, shared);
+                allow_shared<loss_long_kernel<T>>(shared);
                 loss_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 8), kLongThreads, shared, s>>>(a, rows, x, g);
             }
         });

@@ -570,7 +570,13 @@ void launch_pairs(int tile_rows, int64_t rows, int64_t n, int64_t k, const int8_
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    static bool configured[64] = {false};
+    int dev = 0;
+    AFB_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !configured[dev]) {
+        AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        if (dev < 64) configured[dev] = true;
+    }
     AFB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<O>, map_w, map_q, map_y, tile_rows, (int)rows, (int)n, (int)k, q_scale, w_scale,
                                 bias, y, ld_y, n_tma, status));
 }

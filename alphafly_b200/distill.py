@@ -85,48 +85,55 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=Non
     return out
 
 
+class _Loss:
+    """The arguments of one ``afb_distill_loss``, all but the student's logits."""
+
+    def __init__(self, values, moves, log_rest, temperature, legal, weight, scale):
+        self.tensors = [t for t in (values, moves, log_rest, legal[0], legal[1], weight) if t is not None]   # for the backward
+        self.versions = [t._version for t in self.tensors]
+        self.front = (values.shape[1], values.data_ptr(), moves.data_ptr(), _ptr(log_rest), temperature, _ptr(legal[0]),
+                      _ptr(legal[1]), legal[2], _ptr(weight), scale)
+
+    def launch(self, logits, upstream, skip_ones, rows, total, grad) -> None:
+        b, n = logits.shape
+        dev = logits.device
+        with _lib.on_device(dev):
+            _lib.call("afb_distill_loss", b, n, TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), *self.front,
+                      _ptr(upstream), upstream.stride(0) if upstream is not None and upstream.dim() else 0, skip_ones, _ptr(rows),
+                      _ptr(total), _ptr(grad), n, _lib.stream_of(dev))
+
+
 class _Distillation(torch.autograd.Function):
     """The forward writes the gradient for an upstream gradient of 1 in the same pass over the logits.  The backward
     recomputes the rows whose upstream gradient, read on the device, is anything else (it rounds to the logits' type
     once, after the scaling); a second backward writes a gradient of its own."""
 
     @staticmethod
-    def forward(ctx, logits, values, moves, log_rest, temperature, legal_moves, legal_valid, weight, reduction, differentiable):
-        b, n = logits.shape
-        dev = logits.device
-        scale = 1.0 / b if reduction == "mean" and b else 1.0
-        rows = torch.empty(b, dtype=torch.float32, device=dev)
-        total = torch.empty((), dtype=torch.float32, device=dev) if reduction != "none" else None
-        grad = torch.empty(b, n, dtype=logits.dtype, device=dev) if differentiable else None
-        ctx.args = (temperature, scale)
-        ctx.save_for_backward(logits, values, moves, log_rest, legal_moves, legal_valid, weight)
-        ctx.grad = grad
-        _Distillation.launch(ctx.args, logits, values, moves, log_rest, legal_moves, legal_valid, weight, None, 0, False, rows, total, grad)
+    def forward(ctx, logits, loss, reduction, differentiable):
+        b = logits.shape[0]
+        rows = torch.empty(b, dtype=torch.float32, device=logits.device)
+        total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=logits.device)
+        grad = None
+        if differentiable:
+            grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+            ctx.save_for_backward(logits)
+            ctx.loss, ctx.grad = loss, grad
+        loss.launch(logits, None, 0, rows, total, grad)
         return rows if total is None else total
 
     @staticmethod
-    def launch(args, logits, values, moves, log_rest, legal_moves, legal_valid, weight, upstream, step, skip_ones, rows, total, grad):
-        temperature, scale = args
-        b, n = logits.shape
-        dev = logits.device
-        with _lib.on_device(dev):
-            _lib.call("afb_distill_loss", b, n, TYPES[logits.dtype], logits.data_ptr(), logits.stride(0), values.shape[1],
-                      values.data_ptr(), moves.data_ptr(), _ptr(log_rest), temperature, _ptr(legal_moves), _ptr(legal_valid),
-                      legal_moves.shape[1] if legal_moves is not None else 0, _ptr(weight), scale, _ptr(upstream), step,
-                      int(skip_ones), _ptr(rows), _ptr(total), _ptr(grad), n, _lib.stream_of(dev))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g):
+        if torch.is_grad_enabled():
+            raise RuntimeError("distillation_loss has no second derivative (create_graph)")
+        logits, = ctx.saved_tensors
+        if [t._version for t in ctx.loss.tensors] != ctx.loss.versions:
+            raise RuntimeError("distillation_loss: a target or list was modified in place before the backward")
         grad, ctx.grad = ctx.grad, None
-        fresh = grad is None
-        logits = ctx.saved_tensors[0]
-        if fresh:
+        skip = grad is not None
+        if not skip:
             grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        g = g.float()
-        step = 0 if g.dim() == 0 else g.stride(0)
-        _Distillation.launch(ctx.args, *ctx.saved_tensors, g, step, not fresh, None, None, grad)
-        return (grad,) + (None,) * 9
+        ctx.loss.launch(logits, g if g.dtype == torch.float32 else g.float(), int(skip), None, None, grad)
+        return grad, None, None, None
 
 
 def distillation_loss(logits: torch.Tensor, top: TopLogits, legal=None, rest: bool = False, weight: torch.Tensor | None = None,
@@ -146,8 +153,8 @@ def distillation_loss(logits: torch.Tensor, top: TopLogits, legal=None, rest: bo
     values = _matrix(top.values, (b, k), torch.float32, dev, "top.values")
     moves = _matrix(top.moves, (b, k), torch.int64, dev, "top.moves")
     log_rest = _matrix(top.log_rest, (b,), torch.float32, dev, "top.log_rest") if rest else None
-    legal_moves, legal_valid, _ = _legal(legal, logits)
     if weight is not None:
         weight = _matrix(weight.detach(), (b,), torch.float32, dev, "weight")
-    return _Distillation.apply(logits, values, moves, log_rest, float(top.temperature), legal_moves, legal_valid, weight, reduction,
-                               torch.is_grad_enabled() and logits.requires_grad)
+    loss = _Loss(values, moves, log_rest, float(top.temperature), _legal(legal, logits), weight,
+                 1.0 / b if reduction == "mean" and b else 1.0)
+    return _Distillation.apply(logits, loss, reduction, torch.is_grad_enabled() and logits.requires_grad)
