@@ -491,7 +491,7 @@ struct LossArgs {
 // shared memory.
 struct NamedSums {
     float p_rest, log_p_rest;                   // of any other move (0 and -inf without a rest)
-    float ms, log_ss;                           // largest s (0 for -inf), log sum exp((s - ms) / T)
+    float ms, ss, log_ss;                       // largest s (0 for -inf), sum exp((s - ms) / T) and its log
     int some;                                   // a move is named
 };
 struct Named {
@@ -581,7 +581,7 @@ __device__ __forceinline__ void sum_named(const Named &nm, int k, float c) {
     for (int e = lane; e < k; e += 32)
         if (nm.move[e] >= 0) ss += exp2_fast((nm.s[e] - ms) * c);
     ss = warp_reduce(ss, Sum());
-    if (lane == 0) nm.sums->ms = ms, nm.sums->log_ss = logf(ss);
+    if (lane == 0) nm.sums->ms = ms, nm.sums->ss = ss, nm.sums->log_ss = logf(ss);
 }
 
 // The student's log odds of the named moves against the others, whose terms sum to `sum` relative to exp(reference); gap:
@@ -707,34 +707,29 @@ __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_grou
 template <int NT, typename T>
 __device__ __forceinline__ void fetch_row(T *held, const T *row, int n) {
     constexpr int kPer = Piece<T>::kPer;
-    const int shift = shift_of(row), pieces = (shift + n + kPer - 1) / kPer;
-    const bool whole = lead_of(row) == shift;    // pieces of the row start on 16 bytes
-    for (int p = threadIdx.x; p < pieces; p += NT) {
-        const int at = p * kPer - shift;
-        T *const dst = held + p * kPer;
-        if (whole && at >= 0 && at + kPer <= n) {
-            copy_async<16>(dst, row + at);
-            continue;
-        }
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            if (at + e < 0 || at + e >= n) dst[e] = from_float<T>(-kInf);
-            else if (sizeof(T) == 4) copy_async<4>(dst + e, row + at + e);
-            else dst[e] = row[at + e];
-        }
+    const int shift = shift_of(row), whole = (shift + n) / kPer;         // pieces that end within the row
+    if (lead_of(row) == shift) {                 // pieces start on 16 bytes: the first is whole without a shift
+        const T *const from = row - shift;
+        for (int p = (shift ? 1 : 0) + (int)threadIdx.x; p < whole; p += NT) copy_async<16>(held + p * kPer, from + p * kPer);
+        if (shift && threadIdx.x < kPer)
+            held[threadIdx.x] = (int)threadIdx.x >= shift && (int)threadIdx.x < shift + n ? from[threadIdx.x] : from_float<T>(-kInf);
+    } else {
+        for (int m = threadIdx.x; m < whole * kPer; m += NT) copy_async<4>(held + m, row + m);
     }
+    const int m = max(whole, shift ? 1 : 0) * kPer + (int)threadIdx.x;   // the last piece, where it is not whole
+    if (threadIdx.x < kPer) held[m] = m < shift + n ? row[m - shift] : from_float<T>(-kInf);
     asm volatile("cp.async.commit_group;\n" ::: "memory");
 }
 
 // Over all moves, rows held in shared memory, NT threads a row.  The CTAs stay: with kAhead a CTA's next row is on its way
 // (into a second buffer) while it works on one, so that only shared memory is waited for.  The named moves are taken out
-// of the row (-inf), so that its sum is the rest's.  The terms are relative to the student's best named move: no maximum
-// is taken, one barrier joins the sums.  A sum outside kSmall .. kLarge (a rest 69 T from that move, no such move, NaN,
-// values whose product with 1 / T overflows) is taken again, after subtracting the largest.
+// of the row (-inf), so that its sum is the rest's.  The terms are relative to the teacher's best move: no maximum is
+// taken, one barrier joins the sums.  Sums outside kSmall .. kLarge (logits 69 T from that move's, no such move, NaN,
+// values whose product with 1 / T overflows) are taken again, after subtracting the largest.
 constexpr float kSmall = 1e-30f, kLarge = 1e30f;
 
 template <typename T, int NT, bool kAhead>
-__global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, int held_bytes, const T *__restrict__ logits,
+__global__ void __launch_bounds__(NT, 768 / NT) loss_kernel(LossArgs a, int64_t rows, int held_bytes, const T *__restrict__ logits,
                                                   T *__restrict__ grad) {
     constexpr int kPer = Piece<T>::kPer;
     constexpr bool kKeep = sizeof(T) == 4;      // the terms replace the logits in shared memory
@@ -777,10 +772,7 @@ __global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, int 
                        return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u);
                    });
         if (after < rows) first_named = FirstNamed(a, after);
-        float ref = -kInf;                      // every warp for itself
-        for (int e = lane; e < a.k; e += 32)
-            if (nm.move[e] >= 0) ref = fmaxf(ref, nm.s[e]);
-        ref = warp_reduce(ref, Max()) * c;      // a term is 2^(s c - ref): one rounding of the exponent
+        const float ref = nm.s[0] * c;          // a term is 2^(s c - ref): one rounding of the exponent
         float sum = 0.f;
 #pragma unroll 4
         for (int p = threadIdx.x; p < pieces; p += NT) {
@@ -802,11 +794,45 @@ __global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, int 
         sum = 0.f;
 #pragma unroll
         for (int w = 0; w < NT / 32; ++w) sum += scratch[w];
-        const float weight = a.weight ? a.weight[i] : 1.f, f = a.temperature * a.scale * weight * (a.upstream ? a.upstream[i * a.upstream_step] : 1.f);
-        const bool again = !(sum > kSmall && sum < kLarge);
-        float gap = fmaf(nm.sums->ms, c, -ref) * kLn2, base = -kInf;
-        if (again) {
+        const float weight = a.weight ? a.weight[i] : 1.f;
+        const float f = a.temperature * a.scale * weight * (a.upstream ? a.upstream[i * a.upstream_step] : 1.f);
+        // the named moves' terms, and all
+        const float to_ref = exp2_fast(fmaf(nm.sums->ms, c, -ref)), named = nm.sums->ss * to_ref, total = sum + named;
+        if (sum > kSmall && named > kSmall && total < kLarge) {
+            if (a.loss && warp == 0) {
+                const float log_total = logf(total);
+                float part = 0.f;
+                for (int e = lane; e < a.k; e += 32)
+                    if (nm.move[e] >= 0 && !(nm.p[e] == 0.f)) part += nm.p[e] * (nm.z[e] - (fmaf(nm.s[e], c, -ref) * kLn2 - log_total));
+                part = warp_reduce(part, Sum());
+                if (!(nm.sums->p_rest == 0.f)) part += nm.sums->p_rest * (nm.sums->log_p_rest + log1pf(named / sum));
+                if (lane == 0) a.loss[i] = part * (a.temperature * a.temperature) * weight;
+            }
+            if (g) {
+                // outside the named moves: the softmax, less the teacher's rest spread like the student's
+                const float per_term = f * (__fdividef(1.f, total) - __fdividef(nm.sums->p_rest, sum));
+                auto gradient = [&](T v) { return from_float<T>(per_term * (kKeep ? to_float(v) : exp2_fast(fmaf(to_float(v), c, -ref)))); };
+                if (lead_of(g) == shift) {
+#pragma unroll 4
+                    for (int p = threadIdx.x; p < pieces; p += NT) {
+                        Piece<T> v;
+                        v.raw = *reinterpret_cast<const uint4 *>(held + p * kPer);
+#pragma unroll
+                        for (int e = 0; e < kPer; ++e) v.e[e] = gradient(v.e[e]);
+                        store_piece(g, p * kPer - shift, n, v);
+                    }
+                } else {
+                    for (int m = threadIdx.x; m < n; m += NT) g[m] = gradient(held[shift + m]);
+                }
+                __syncthreads();
+                for (int e = threadIdx.x; e < a.k; e += NT)
+                    if (nm.move[e] >= 0)
+                        g[nm.move[e]] = from_float<T>(f * (__fdividef(exp2_fast(fmaf(nm.s[e], c, -ref)), total) - nm.p[e]));
+            }
+        } else {
+            // rare: the row again, its largest values subtracted, the shares by their log odds
             __syncthreads();
+            float base = -kInf;
             for (int m = threadIdx.x; m < n; m += NT) {
                 held[shift + m] = (marks[m >> 5] >> (m & 31)) & 1u ? from_float<T>(-kInf) : row[m];
                 base = fmaxf(base, to_float(held[shift + m]));
@@ -814,37 +840,17 @@ __global__ void __launch_bounds__(NT) loss_kernel(LossArgs a, int64_t rows, int 
             base = block_reduce(base, scratch, -kInf, Max());
             base = base > -kInf ? base : 0.f;
             sum = 0.f;
-            for (int m = threadIdx.x; m < n; m += NT) {
-                const float x = exp2_fast((to_float(held[shift + m]) - base) * c);
-                if constexpr (kKeep) held[shift + m] = x;
-                sum += x;
-            }
+            for (int m = threadIdx.x; m < n; m += NT) sum += exp2_fast((to_float(held[shift + m]) - base) * c);
             sum = block_reduce(sum, scratch, 0.f, Sum());
-            gap = (nm.sums->ms - base) * inv_t;
-        }
-        const float odds = odds_of(nm, gap, sum);
-        if (a.loss && warp == 0) write_loss(nm, a, i, odds, sum, inv_t, weight);
-        if (g) {
-            const float beyond = beyond_of(nm, odds, sum, f);
-            auto gradient = [&](T v) {
-                const float s = to_float(v);
-                if (again) return from_float<T>(times(beyond, kKeep ? s : exp2_fast((s - base) * c)));
-                return from_float<T>(beyond * (kKeep ? s : exp2_fast(fmaf(s, c, -ref))));
-            };
-            if (lead_of(g) == shift) {
-#pragma unroll 4
-                for (int p = threadIdx.x; p < pieces; p += NT) {
-                    Piece<T> v;
-                    v.raw = *reinterpret_cast<const uint4 *>(held + p * kPer);
-#pragma unroll
-                    for (int e = 0; e < kPer; ++e) v.e[e] = gradient(v.e[e]);
-                    store_piece(g, p * kPer - shift, n, v);
-                }
-            } else {
-                for (int m = threadIdx.x; m < n; m += NT) g[m] = gradient(held[shift + m]);
+            const float odds = odds_of(nm, (nm.sums->ms - base) * inv_t, sum);
+            if (a.loss && warp == 0) write_loss(nm, a, i, odds, sum, inv_t, weight);
+            if (g) {
+                const float beyond = beyond_of(nm, odds, sum, f);
+                for (int m = threadIdx.x; m < n; m += NT)
+                    g[m] = from_float<T>(times(beyond, exp2_fast((to_float(held[shift + m]) - base) * c)));
+                __syncthreads();
+                write_named(nm, a.k, odds, sum, inv_t, f, g);
             }
-            __syncthreads();
-            write_named(nm, a.k, odds, sum, inv_t, f, g);
         }
         for (int e = threadIdx.x; e < a.k; e += NT)
             if (nm.move[e] >= 0) marks[nm.move[e] >> 5] = 0u;
@@ -988,6 +994,23 @@ void allow_shared(size_t bytes) {
     if (dev < 64) allowed[dev] = bytes;
 }
 
+// CTAs of a kernel that the current device holds at once (asked for again when the shared memory changes).
+template <auto kKernel>
+int64_t resident(int threads, size_t shared) {
+    static size_t of[64] = {0};
+    static int64_t ctas[64] = {0};
+    int dev = 0;
+    AFB_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && ctas[dev] && of[dev] == shared) return ctas[dev];
+    int per_sm = 0, sms = 0;
+    AFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, threads, shared));
+    AFB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    AFB_CHECK(per_sm >= 1, "the kernel does not fit on this device");
+    const int64_t n = (int64_t)per_sm * sms;
+    if (dev < 64) of[dev] = shared, ctas[dev] = n;
+    return n;
+}
+
 void check_rows(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k, float temperature,
                 const int64_t *list, const uint8_t *valid, int64_t n_listed) {
     AFB_CHECK(rows >= 0 && n_moves >= 0 && n_listed >= 0, "negative size");
@@ -1077,9 +1100,7 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
                 constexpr auto kernel = loss_kernel<T, NT, decltype(ahead)::value>;
                 const size_t shared = (decltype(ahead)::value ? 2 : 1) * held + more;
                 allow_shared<kernel>(shared);
-                // as many CTAs as the device holds: 228 KB of shared memory an SM, of which a CTA takes 1.2 KB besides
-                const int64_t ctas = std::min<int64_t>(2048 / NT, 228 * 1024 / (shared + 1280));
-                kernel<<<(unsigned)std::min<int64_t>(rows, 148 * ctas), NT, shared, s>>>(a, rows, (int)held, x, g);
+                kernel<<<(unsigned)std::min<int64_t>(rows, resident<kernel>(NT, shared)), NT, shared, s>>>(a, rows, (int)held, x, g);
             };
             if (held <= 20 * 1024) go(std::integral_constant<int, 128>{}, std::true_type{});
             else if (held <= 36 * 1024) go(std::integral_constant<int, 256>{}, std::true_type{});
@@ -1087,7 +1108,7 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
             else {
                 const size_t shared = more;
                 allow_shared<loss_long_kernel<T>>(shared);
-                loss_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 8), kLongThreads, shared, s>>>(a, rows, x, g);
+                loss_long_kernel<T><<<(unsigned)std::min<int64_t>(rows, resident<loss_long_kernel<T>>(kLongThreads, shared)), kLongThreads, shared, s>>>(a, rows, x, g);
             }
         });
         AFB_LAUNCHED();
