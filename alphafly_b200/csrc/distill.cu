@@ -917,18 +917,26 @@ __global__ void __launch_bounds__(kLongThreads) loss_long_kernel(LossArgs a, int
                 }
             }
         };
-        float m = -kInf, sum = 0.f;
-        each([&](const Piece<T> &v, int) {
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) m = fmaxf(m, to_float(v.e[e]));
-        });
-        m = block_reduce(m, scratch, -kInf, Max());
-        const float base = m > -kInf ? m : 0.f;
-        each([&](const Piece<T> &v, int) {
+        // as above: relative to the teacher's best move, or, where that does not do, to the largest
+        float base = nm.s[0] > -kInf ? nm.s[0] : 0.f, sum = 0.f;
+        auto add = [&](const Piece<T> &v, int) {
 #pragma unroll
             for (int e = 0; e < kPer; ++e) sum += exp2_fast((to_float(v.e[e]) - base) * c);
-        });
+        };
+        each(add);
         sum = block_reduce(sum, scratch, 0.f, Sum());
+        if (!(sum > kSmall && sum < kLarge)) {
+            base = -kInf;
+            each([&](const Piece<T> &v, int) {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) base = fmaxf(base, to_float(v.e[e]));
+            });
+            base = block_reduce(base, scratch, -kInf, Max());
+            base = base > -kInf ? base : 0.f;
+            sum = 0.f;
+            each(add);
+            sum = block_reduce(sum, scratch, 0.f, Sum());
+        }
         const float weight = a.weight ? a.weight[i] : 1.f, f = a.temperature * a.scale * weight * up;
         const float odds = odds_of(nm, (nm.sums->ms - base) * inv_t, sum);
         if (a.loss && warp == 0) write_loss(nm, a, i, odds, sum, inv_t, weight);
