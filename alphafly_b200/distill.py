@@ -10,6 +10,9 @@ position's k best policy logits of the teacher, some 12 k bytes instead of a den
 with p = softmax(teacher / T) over the k named moves and, with ``rest``, one more outcome "any other move" of
 the mass the teacher leaves to it, and q = softmax(student / T) over all moves or the legal ones.  Both run in
 libafb (``afb_top_logits``, ``afb_distill_loss``); the loss and its gradient are one pass over the logits.
+
+    top = teacher_targets(teacher, batch.x, 16, legal=(batch.moves, batch.valid))      # teacher.infer_heads = "int8"
+    train_step(student, opt, batch, device, teacher=top)                               # alphafly_b200.train
 """
 
 from __future__ import annotations
@@ -83,6 +86,19 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=Non
                   _ptr(moves), _ptr(valid), listed, out.values.data_ptr(), out.moves.data_ptr(), out.log_rest.data_ptr(),
                   _lib.stream_of(dev))
     return out
+
+
+@torch.no_grad()
+def teacher_targets(teacher, x: torch.Tensor, k: int, temperature: float = 1.0, legal=None) -> TopLogits:
+    """``teacher`` (a ``FlyChessNet``) on the positions ``x`` (B, N_FEATURES), in inference: its ``top_logits``.  With
+    ``teacher.infer_heads`` "int8" the readout runs in 8-bit integers."""
+    mode = teacher.training
+    teacher.eval()
+    try:
+        logits, _ = teacher(x)
+    finally:
+        teacher.train(mode)
+    return top_logits(logits, k, temperature, legal)
 
 
 class _Loss:

@@ -10,8 +10,8 @@ load unchanged.  The recurrence runs in ``alphafly_b200.brain`` (libafb).  The i
 instead of x W^T followed by a transpose copy: for float16 inference in libafb's tensor-core kernel
 (``input_map_f16``), in float32 (training, the float32 path) through cuBLAS.  In inference the normaliser
 and the heads are one tensor-core readout in libafb (``FlyChessNet.heads``: the factorised from/to terms
-folded into the policy rows, float32 accuracy from split float16 operands); training keeps the float32
-layers, whose gradients autograd takes.
+folded into the policy rows, float32 accuracy from split float16 operands, or 8-bit products with
+``infer_heads`` "int8"); training keeps the float32 layers, whose gradients autograd takes.
 """
 
 from __future__ import annotations
@@ -28,6 +28,7 @@ from .brain import ConnectomeRNN
 from .connectome import Connectome
 from .encoding import N_BASE, N_FEATURES, N_MOVES, move_squares
 from .gemm import affine, status_word
+from .int8 import int8_linear, quantize
 
 READOUT_SUPERCLASSES = ("descending_neuron",)   # plus every efferent neuron (chessfly/model.py:23)
 
@@ -75,6 +76,8 @@ class FlyChessNet(nn.Module):
         self.cfg = cfg
         # float16 inference is the deviation form (brain.forward_io with float16 input), as in the reference
         self.infer_dtype = torch.float16
+        # the readout of inference: "float32" (accuracy), or "int8" (8-bit products, for a teacher over a large pool)
+        self.infer_heads = "float32"
         if cfg.shuffled:
             conn = conn.shuffled()
         self.brain = ConnectomeRNN(conn, bias_init=cfg.bias_init, global_scale=cfg.weight_scale)
@@ -180,8 +183,16 @@ class FlyChessNet(nn.Module):
         normaliser in eval mode runs the normaliser and the heads as one tensor-core readout (``heads``);
         training (and a normaliser still collecting statistics) keeps the float32 layers."""
         if x.is_cuda and not torch.is_grad_enabled() and not self.norm.training:
-            return self.heads(self.brain_output(x))
+            return self.inference_heads(self.brain_output(x))
         return self.dense_heads(self.readout(x))
+
+    def inference_heads(self, out: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """The recurrence's output (len(out_idx), B) -> policy and WDL logits by the readout ``infer_heads`` names."""
+        if self.infer_heads == "int8":
+            return self.int8_heads(out)
+        if self.infer_heads != "float32":
+            raise ValueError(f"infer_heads must be 'float32' or 'int8', not {self.infer_heads!r}")
+        return self.heads(out)
 
     def dense_heads(self, r: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """The heads as the reference's float32 layers on the normalised state r (B, len(out_idx))
@@ -200,6 +211,45 @@ class FlyChessNet(nn.Module):
         logits = torch.addmm(policy, ft, self.move_select)
         return logits, self.value(r)
 
+    def _folded(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(weight, bias) of the policy with the factorised from/to terms folded in, and the value rows below it."""
+        w = torch.cat([self.policy.weight + self.policy_from.weight[self.move_from] + self.policy_to.weight[self.move_to],
+                       self.value.weight]).float().contiguous()
+        b = torch.cat([self.policy.bias + self.policy_from.bias[self.move_from] + self.policy_to.bias[self.move_to],
+                       self.value.bias]).float().contiguous()
+        return w, b
+
+    @torch.no_grad()
+    def quantized_heads(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """(q, scale, bias) of the 8-bit readout: the folded rows in int8 with a float32 scale each
+        (``int8.quantize``), and the float32 bias.  Rewritten in place when a head parameter changed, so a captured
+        CUDA graph reading them stays valid."""
+        layers = (self.policy, self.policy_from, self.policy_to, self.value)
+        params = [t for layer in layers for t in (layer.weight, layer.bias)]
+        key = tuple(t._version for t in params)
+        where = tuple(t.data_ptr() for t in params)
+        c = getattr(self, "_heads8", None)
+        if c is not None and c[0] == key and c[1] == where:
+            return c[2]
+        w, b = self._folded()
+        new = (*quantize(w), b)
+        if c is not None and c[1] == where:
+            for old, t in zip(c[2], new):
+                old.copy_(t)
+            new = c[2]
+        self._heads8 = (key, where, new)
+        return new
+
+    @torch.no_grad()
+    def int8_heads(self, out: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """``heads`` in 8-bit integers: the normalised state with a scale per position, the folded rows with a scale
+        each, exact sums (``int8.int8_linear``; the normaliser runs in its quantisation).  An entry of the state is off by
+        up to half a step of its position (largest / 127), a weight by half a step of its row.  Views of one result, rows
+        on 16 bytes."""
+        q, scale, bias = self.quantized_heads()
+        y = int8_linear(out.T, q, scale, bias, norm=self.norm)
+        return y[:, :N_MOVES], y[:, N_MOVES:]
+
     @torch.no_grad()
     def folded_heads(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """(W_hi, W_lo, bias) of the tensor-core readout: the policy rows with the factorised from/to terms
@@ -213,10 +263,7 @@ class FlyChessNet(nn.Module):
         c = getattr(self, "_heads16", None)
         if c is not None and c[0] == key and c[1] == where:
             return c[2], c[3], c[4]
-        w = torch.cat([self.policy.weight + self.policy_from.weight[self.move_from] + self.policy_to.weight[self.move_to],
-                       self.value.weight]).float().contiguous()
-        b = torch.cat([self.policy.bias + self.policy_from.bias[self.move_from] + self.policy_to.bias[self.move_to],
-                       self.value.bias]).float().contiguous()
+        w, b = self._folded()
         rows, n_out = w.shape
         ldw = -(-n_out // 8) * 8
         if c is None or c[1] != where or c[2].shape != (rows, ldw):
@@ -321,7 +368,7 @@ class Evaluator:
         captured once per batch bucket (multiples of 256 positions, the step kernel's batch tile; at most
         ``max_graphs`` kept); the weight-dependent constants are refreshed before a replay when a
         parameter changed, so training between rounds is seen;
-      - the readout is libafb's tensor-core kernel (``FlyChessNet.heads``, part of the graph): the dense
+      - the readout is libafb's tensor-core kernel (``FlyChessNet.inference_heads``, part of the graph): the dense
         (B, 4168) logits at float32 accuracy, from which the legal entries are gathered, or which are
         rounded to float16 for the lazy search.
     """
@@ -359,7 +406,7 @@ class Evaluator:
         """Features -> (policy logits (B, N_MOVES) float32, values (B,)): the recurrence and the tensor-core
         readout."""
         net = self.net
-        logits, wdl = net.heads(net.brain_output(x))
+        logits, wdl = net.inference_heads(net.brain_output(x))
         return logits, net.expected_value(wdl)
 
     def _refresh_constants(self) -> None:
@@ -367,12 +414,12 @@ class Evaluator:
         mode = _lib.MODE_DEV16 if net.infer_dtype == torch.float16 else _lib.MODE_F32
         if mode == _lib.MODE_DEV16:
             net.half_encoder()
-        net.folded_heads()
+        net.quantized_heads() if net.infer_heads == "int8" else net.folded_heads()
         cone = brain.light_cone(net.in_idx, net.out_idx, net.cfg.steps)
         cone.set_weights(brain, mode, brain._weight_key(mode, cone))
 
     def _graph(self, bucket: int):
-        key = (bucket, self.net.infer_dtype)
+        key = (bucket, self.net.infer_dtype, self.net.infer_heads)
         entry = self._graphs.get(key)
         if entry is not None:
             self._graphs.move_to_end(key)
@@ -496,7 +543,7 @@ class ShardedEvaluator:
         self.replicas = []
         for d in self.devices:
             r = copy.deepcopy(net).to(d)
-            r.infer_dtype = net.infer_dtype
+            r.infer_dtype, r.infer_heads = net.infer_dtype, net.infer_heads
             self.replicas.append(r)
         self.evaluators = [Evaluator(r, d, graphs=graphs, max_graphs=max_graphs) for r, d in zip(self.replicas, self.devices)]
 
@@ -508,7 +555,7 @@ class ShardedEvaluator:
                 s = src[k]
                 if not torch.equal(t.detach(), s.detach().to(t.device)):
                     t.detach().copy_(s.detach())
-            r.infer_dtype = self.net.infer_dtype
+            r.infer_dtype, r.infer_heads = self.net.infer_dtype, self.net.infer_heads
 
     def submit(self, x, rows, cols):
         b = len(x)

@@ -26,6 +26,7 @@ from typing import NamedTuple
 import numpy as np
 import torch
 
+from .distill import TopLogits, distillation_loss
 from .model import FlyChessNet
 
 
@@ -155,11 +156,20 @@ def value_losses(wdl_logits: torch.Tensor, batch: Batch, q_ratio: float, reducti
     return (1 - q_ratio) * ce_r + q_ratio * red(sq), ce_r
 
 
-def loss_terms(net: FlyChessNet, batch: Batch, q_ratio: float):
-    """The forward pass of a training step: (policy loss, value loss, WDL cross-entropy)."""
+def loss_terms(net: FlyChessNet, batch: Batch, q_ratio: float, teacher: TopLogits | None = None, teacher_share: float = 1.0,
+               teacher_rest: bool = False):
+    """The forward pass of a training step: (policy loss, value loss, WDL cross-entropy).  With ``teacher`` the policy
+    loss is ``teacher_share`` of the divergence from the teacher's best moves over the legal ones
+    (``distill.distillation_loss``; ``teacher_rest``: its other moves count as one) and the cross-entropy for the
+    remaining share."""
     logits, wdl_logits = net(batch.x)
     value, ce = value_losses(wdl_logits, batch, q_ratio)
-    return policy_cross_entropy(logits, batch), value, ce
+    if teacher is None:
+        return policy_cross_entropy(logits, batch), value, ce
+    policy = distillation_loss(logits, teacher, legal=(batch.moves, batch.valid), rest=teacher_rest)
+    if teacher_share != 1.0:
+        policy = teacher_share * policy + (1.0 - teacher_share) * policy_cross_entropy(logits, batch)
+    return policy, value, ce
 
 
 def grow_optimizer_state(opt_state: dict, opt: torch.optim.Optimizer) -> dict:
@@ -327,13 +337,15 @@ def attach_data_parallel(net: FlyChessNet, group=None, bucket_mb: float = 25.0) 
 
 
 def train_step(net, opt, batch, device, q_ratio: float = 0.0, policy_target_offset: float = 0.0,
-               data_parallel: bool = False, group=None) -> dict:
+               data_parallel: bool = False, group=None, teacher: TopLogits | None = None, teacher_share: float = 1.0,
+               teacher_rest: bool = False) -> dict:
     """One optimisation step (chessfly/train.py:126-138): losses, backward, clip at 5, AdamW.  ``batch`` is a
     list of ``Sample`` or a ``Batch`` already on the device; ``data_parallel`` averages the gradients over the
-    process group before clipping (the batch is this rank's share)."""
+    process group before clipping (the batch is this rank's share).  ``teacher``: another network's best moves of
+    the batch's positions, to learn the policy from (``loss_terms``)."""
     if not isinstance(batch, Batch):
         batch = make_batch(batch, device, policy_target_offset)
-    policy_loss, value_loss, value_ce = loss_terms(net, batch, q_ratio)
+    policy_loss, value_loss, value_ce = loss_terms(net, batch, q_ratio, teacher, teacher_share, teacher_rest)
     opt.zero_grad(set_to_none=True)
     reducer = getattr(net, "grad_reducer", None) if data_parallel else None
     if reducer is not None and reducer.group is group:
