@@ -11,6 +11,7 @@
 // and product in one launch), pair_kernel for the rest, on the tensor cores.  The largest magnitude of a row is an
 // integer maximum of the magnitudes' bits, which order like the magnitudes and put NaN on top.
 #include <cstring>
+#include <type_traits>
 
 #include "dtypes.cuh"
 #include "tc.cuh"
@@ -25,13 +26,18 @@ constexpr unsigned kInfBits = 0x7f800000u;
 __device__ __forceinline__ float row_scale(unsigned amax_bits) {
     return amax_bits >= kInfBits ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(amax_bits), kTop);
 }
-// rint(fl(x / scale)) as a byte, by the division.  The quotient is within 127 (1 + 2^-23) unless the scale is subnormal,
-// where it can round further up.  0 for a scale of 0 or NaN.
-__device__ __noinline__ uint32_t quantize_by_division(float x, float scale) {
-    if (!(scale > 0.f)) return 0u;
-    return (uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x, scale)), -kTop), kTop) & 0xffu;
+// Four rint(fl(x / scale)) as bytes, by the division.  The quotient is within 127 (1 + 2^-23) unless the scale is
+// subnormal, where it can round further up.  0 for a scale of 0 or NaN.
+__device__ __noinline__ uint32_t quantize4_by_division(float x0, float x1, float x2, float x3, float scale) {
+    const float x[4] = {x0, x1, x2, x3};
+    uint32_t word = 0u;
+    if (scale > 0.f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            word |= ((uint32_t)(int)fminf(fmaxf(rintf(__fdiv_rn(x[e], scale)), -kTop), kTop) & 0xffu) << (8 * e);
+    return word;
 }
-// Four of them with inv = fl(1 / scale).  t = x inv is off x / scale by less than 1.6e-5 (127 times two roundings), the
+// The same with inv = fl(1 / scale).  t = x inv is off x / scale by less than 1.6e-5 (127 times two roundings), the
 // rounded quotient by 7.6e-6: unless t lies within 4e-5 of a half, both round to the same whole number, which
 // t + 1.5 2^23 holds in its low bits.  One element in 12,000 takes the division, and so do the scales whose reciprocal
 // is infinite and rows without one (inv NaN).  Rounding and conversion instructions run at a quarter of the rate.
@@ -46,9 +52,7 @@ __device__ __forceinline__ uint32_t quantize4(float x0, float x1, float x2, floa
         f[e] = t + kMagic;
         near |= !(fabsf(t - (f[e] - kMagic)) < 0.49996f);
     }
-    if (near)
-        return quantize_by_division(x0, scale) | quantize_by_division(x1, scale) << 8 | quantize_by_division(x2, scale) << 16 |
-               quantize_by_division(x3, scale) << 24;
+    if (near) return quantize4_by_division(x0, x1, x2, x3, scale);
     return __byte_perm(__byte_perm(__float_as_uint(f[0]), __float_as_uint(f[1]), 0x0040),
                        __byte_perm(__float_as_uint(f[2]), __float_as_uint(f[3]), 0x0040), 0x5410);
 }
@@ -66,16 +70,36 @@ struct Norm {
     }
 };
 
+// The largest magnitude of the values it was given, as bits; 16-bit types two at a time (NaN stays).
+template <typename T>
+struct LargestOf {
+    using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    Two two;
+    __device__ __forceinline__ LargestOf() { two.x = two.y = from_float<T>(0.f); }
+    __device__ __forceinline__ void add(const Piece<T> &v) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) two = __hmax2_nan(two, __habs2(*reinterpret_cast<const Two *>(&v.e[2 * h])));
+    }
+    __device__ __forceinline__ unsigned bits() const { return max(magnitude(to_float(two.x)), magnitude(to_float(two.y))); }
+};
+template <>
+struct LargestOf<float> {
+    unsigned m = 0u;
+    __device__ __forceinline__ void add(const Piece<float> &v) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = max(m, magnitude(v.e[e]));
+    }
+    __device__ __forceinline__ unsigned bits() const { return m; }
+};
+
 constexpr int kRowThreads = 128;
-constexpr int kRowPieces = 8;                    // most 16-byte pieces a thread keeps
 
 // One CTA per row of x (element (i, k) at x[i ld + k]), P pieces a thread.  The row is read in 16-byte pieces wherever it
-// starts and, up to 4,080 float32 or 8,176 16-bit elements, kept in registers (longer rows are read again, from cache); the quantised
+// starts and, where the CTA's pieces hold it, kept in registers (longer rows are read again, from cache); the quantised
 // bytes are shifted to their place through shared memory and leave as 16-byte words, zero past k.
 template <typename T, int P>
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int64_t k_dim, const T *__restrict__ x, int64_t ld, Norm norm,
-                                                                    int8_t *__restrict__ q, int64_t ld_q,
-                                                                    float *__restrict__ scale) {
+__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int k_dim, const T *__restrict__ x, int64_t ld, Norm norm,
+                                                                    int8_t *__restrict__ q, int64_t ld_q, float *__restrict__ scale) {
     constexpr int kPer = Piece<T>::kPer, kSpan = kRowThreads * P * kPer;
     constexpr int kStep = kSpan - 16;            // elements a span writes: it starts up to 7 before its first
     __shared__ unsigned amax;
@@ -83,40 +107,43 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int64_t k_di
     const int64_t i = blockIdx.x;
     const T *row = x + i * ld;
     const int lead = lead_of(row);
+    Piece<T> mine[P];
+    auto first_of = [&](int base, int p) { return base + ((int)threadIdx.x + p * kRowThreads) * kPer - lead; };
+    auto load = [&](int base) {                  // the pieces from element base - lead on
+#pragma unroll
+        for (int p = 0; p < P; ++p) mine[p] = first_of(base, p) < k_dim ? load_piece(row, first_of(base, p), k_dim, from_float<T>(0.f)) : Piece<T>();
+    };
+    // with statistics an element takes 32 bits, so it is normalised where it is used
+    auto value = [&](int base, int p, int e) {
+        const float v = to_float(mine[p].e[e]);
+        const int k = first_of(base, p) + e;
+        return norm.mean && k >= 0 && k < k_dim ? norm(v, k) : v;
+    };
     if (threadIdx.x == 0) amax = 0u;
     __syncthreads();
-    Piece<T> mine[P];
-    auto first_of = [&](int64_t base, int p) { return base + (int64_t)(p * kRowThreads + threadIdx.x) * kPer - lead; };
-    auto load = [&](int64_t base) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const int64_t k = first_of(base, p);
-            mine[p] = k < k_dim ? load_piece(row, (int)k, (int)k_dim, from_float<T>(0.f)) : Piece<T>();
-        }
-    };
-    auto value = [&](int64_t base, int p, int e) {
-        const float v = to_float(mine[p].e[e]);
-        if (!norm.mean) return v;
-        const int64_t k = first_of(base, p) + e;
-        return k >= 0 && k < k_dim ? norm(v, k) : 0.f;
-    };
+    LargestOf<T> largest;
     unsigned m = 0u;
-    for (int64_t base = 0; base < k_dim; base += kStep) {
+    for (int base = 0; base < k_dim; base += kStep) {
         load(base);
 #pragma unroll
-        for (int p = 0; p < P; ++p)
+        for (int p = 0; p < P; ++p) {
+            if (norm.mean) {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) m = max(m, magnitude(value(base, p, e)));
+                for (int e = 0; e < kPer; ++e) m = max(m, magnitude(value(base, p, e)));
+            } else {
+                largest.add(mine[p]);
+            }
+        }
     }
-    m = __reduce_max_sync(0xffffffffu, m);
+    m = __reduce_max_sync(0xffffffffu, max(m, largest.bits()));
     if ((threadIdx.x & 31) == 0) atomicMax(&amax, m);
     __syncthreads();
     const float s = row_scale(amax), inv = inverse(s);
     if (threadIdx.x == 0) scale[i] = s;
-    for (int64_t base = 0; base < k_dim; base += kStep) {
+    for (int base = 0; base < k_dim; base += kStep) {
         if (k_dim > kStep) load(base);
 #pragma unroll
-        for (int p = 0; p < P; ++p)                             // byte b of the span: element base - lead + b
+        for (int p = 0; p < P; ++p)                                      // byte b of the span: element base - lead + b
 #pragma unroll
             for (int w = 0; w < kPer / 4; ++w) {
                 uint32_t word = 0u;
@@ -125,90 +152,87 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int64_t k_di
                 bytes[(p * kRowThreads + threadIdx.x) * (kPer / 4) + w] = word;
             }
         __syncthreads();
-        const int n = (int)min((int64_t)kStep, k_dim - base);
+        const int n = min(kStep, k_dim - base), by = 8 * (lead & 3);
         for (int b = threadIdx.x * 16; b < n; b += kRowThreads * 16) {
             uint32_t w[5];
 #pragma unroll
             for (int e = 0; e < 5; ++e) w[e] = bytes[(b + lead) / 4 + e];
-            const int by = 8 * ((b + lead) & 3);
             *reinterpret_cast<uint4 *>(q + i * ld_q + base + b) =
                 make_uint4(__funnelshift_r(w[0], w[1], by), __funnelshift_r(w[1], w[2], by), __funnelshift_r(w[2], w[3], by),
                            __funnelshift_r(w[3], w[4], by));
         }
-        __syncthreads();
+        if (k_dim > kStep) __syncthreads();
     }
 }
 
 constexpr int kColRows = 32;                     // rows of the result per cluster, one per lane
-constexpr int kColCluster = 8;                   // CTAs of a cluster: shares of k
 constexpr int kColWarps = 8;
-constexpr int kColKeep = 40;                     // values a thread keeps
-constexpr int kColSpan = kColWarps * kColKeep;   // 320
+constexpr int kColCluster = 8;                   // most CTAs of a cluster
+constexpr int kColKeep = 40;                     // most values a thread keeps
 
-// The transposed layout: element (i, k) at x[k ld + i], lanes along the rows i.  A cluster of 8 CTAs shares 32 rows,
-// each CTA an eighth of k; the CTAs' largest magnitudes meet through distributed shared memory.  Up to k = 2,560 the
-// values stay in registers (beyond it they are read again, from cache); the bytes are transposed in shared memory.
-template <typename T>
-__global__ void __cluster_dims__(kColCluster, 1, 1) __launch_bounds__(32 * kColWarps)
-    quantize_columns_kernel(int64_t rows, int64_t k_dim, const T *__restrict__ x, int64_t ld, Norm norm, int8_t *__restrict__ q,
+// The transposed layout: element (i, k) at x[k ld + i], lanes along the rows i.  A cluster of up to 8 CTAs shares 32
+// rows, each CTA a part of k; the CTAs' largest magnitudes meet through distributed shared memory.  Up to 320 values of k
+// a CTA stay in registers, V a thread (beyond 2,560 they are read again, from cache); the bytes are transposed in shared
+// memory.
+template <typename T, int V>
+__global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
+    quantize_columns_kernel(int64_t rows, int k_dim, int share, const T *__restrict__ x, int64_t ld, Norm norm, int8_t *__restrict__ q,
                             int64_t ld_q, float *__restrict__ scale) {
+    constexpr int kSpan = kColWarps * V, kWords = kSpan / 4;
     __shared__ unsigned amax[kColRows];
-    __shared__ __align__(16) int8_t tile[kColRows][kColSpan + 16];    // rows 21 words of 16 bytes apart
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t i0 = (int64_t)(blockIdx.x / kColCluster) * kColRows, i = i0 + lane;
-    // this CTA's share of k, in whole 16-byte words
-    const int64_t share = ((k_dim + kColCluster - 1) / kColCluster + 15) / 16 * 16;
-    const int64_t k0 = share * tc::cluster_rank(), k1 = min(k0 + share, k_dim);
+    __shared__ uint32_t tile[kColRows][kWords | 1];                      // an odd pitch: lanes write different banks
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, ctas = (int)tc::cluster_size();
+    const int64_t i0 = (int64_t)(blockIdx.x / ctas) * kColRows, i = i0 + lane;
+    const int k0 = share * (int)tc::cluster_rank(), k1 = min(k0 + share, k_dim);
     if (threadIdx.x < kColRows) amax[threadIdx.x] = 0u;
     __syncthreads();
-    float mine[kColKeep];
-    auto k_of = [&](int p) { return (p / 4 * kColWarps + warp) * 4 + p % 4; };
-    auto load = [&](int64_t base) {
+    const bool in = i < rows;
+    float mine[V];
+    auto k_of = [&](int p) { return (p / 4 * kColWarps + warp) * 4 + p % 4; };   // a thread's fours are neighbours in k
+    auto load = [&](int base) {
 #pragma unroll
-        for (int p = 0; p < kColKeep; ++p) {
-            const int64_t k = base + k_of(p);
-            mine[p] = i < rows && k < k1 ? to_float(x[k * ld + i]) : 0.f;
+        for (int p = 0; p < V; ++p) {
+            const int k = base + k_of(p);
+            mine[p] = in && k < k1 ? to_float(x[k * ld + i]) : 0.f;
         }
         if (norm.mean)
 #pragma unroll
-            for (int p = 0; p < kColKeep; ++p) {
-                const int64_t k = base + k_of(p);
-                if (i < rows && k < k1) mine[p] = norm(mine[p], k);
+            for (int p = 0; p < V; ++p) {
+                const int k = base + k_of(p);
+                if (in && k < k1) mine[p] = norm(mine[p], k);
             }
     };
     unsigned m = 0u;
-    for (int64_t base = k0; base < k1; base += kColSpan) {
+    for (int base = k0; base < k1; base += kSpan) {
         load(base);
 #pragma unroll
-        for (int p = 0; p < kColKeep; ++p) m = max(m, magnitude(mine[p]));
+        for (int p = 0; p < V; ++p) m = max(m, magnitude(mine[p]));
     }
     atomicMax(&amax[lane], m);
-    tc::cluster_sync();
+    if (ctas > 1) tc::cluster_sync();
+    else __syncthreads();
+    m = amax[lane];
     const uint32_t own = (uint32_t)__cvta_generic_to_shared(&amax[lane]);
-    m = 0u;
-#pragma unroll
-    for (int c = 0; c < kColCluster; ++c) {
+    for (int c = 0; c < ctas && ctas > 1; ++c) {
         unsigned v;
         asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(tc::map_to(own, (uint32_t)c)) : "memory");
         m = max(m, v);
     }
     const float s = row_scale(m), inv = inverse(s);
-    if (k0 == 0 && warp == 0 && i < rows) scale[i] = s;
-    for (int64_t base = k0; base < k1; base += kColSpan) {
-        if (share > kColSpan) load(base);
-        __syncthreads();                         // the tile's readers are done
-#pragma unroll
-        for (int p = 0; p < kColKeep; p += 4)    // a thread's four values are neighbours in k
-            *reinterpret_cast<uint32_t *>(&tile[lane][k_of(p)]) = quantize4(mine[p], mine[p + 1], mine[p + 2], mine[p + 3], s, inv);
-        __syncthreads();
-        const int words = (int)((min((int64_t)kColSpan, k1 - base) + 15) / 16);
-        for (int e = threadIdx.x; e < kColRows * words; e += 32 * kColWarps) {
-            const int r = e / words, w = e % words;
-            if (i0 + r < rows)
-                *reinterpret_cast<uint4 *>(q + (i0 + r) * ld_q + base + 16 * w) = *reinterpret_cast<const uint4 *>(&tile[r][16 * w]);
+    if (k0 == 0 && warp == 0 && in) scale[i] = s;
+    for (int base = k0; base < k1; base += kSpan) {
+        if (share > kSpan) {
+            load(base);
+            __syncthreads();                     // the tile's readers are done
         }
+#pragma unroll
+        for (int p = 0; p < V; p += 4) tile[lane][k_of(p) / 4] = quantize4(mine[p], mine[p + 1], mine[p + 2], mine[p + 3], s, inv);
+        __syncthreads();
+        const int words = (min(kSpan, k1 - base) + 15) / 16 * 4;         // whole 16-byte units, zero past k
+        for (int r = warp; r < kColRows && i0 + r < rows; r += kColWarps)
+            for (int w = lane; w < words; w += 32) *reinterpret_cast<uint32_t *>(q + (i0 + r) * ld_q + base + 4 * w) = tile[r][w];
     }
-    tc::cluster_sync();                          // no CTA ends while another may read its maxima
+    if (ctas > 1) tc::cluster_sync();            // no CTA ends while another may read its maxima
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------
@@ -599,27 +623,54 @@ void check_rows16(const void *p, int64_t ld, const char *what) {
     AFB_CHECK((reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 16 == 0, std::string(what) + " rows must start on 16-byte boundaries");
 }
 
+template <typename T>
+void quantize_columns(int64_t rows, int k, const T *x, int64_t ld_x, const Norm &norm, int8_t *q, int64_t ld_q, float *scale, cudaStream_t s) {
+    // as many CTAs a cluster as give each at most the values it can keep
+    int ctas = 1;
+    while (ctas < kColCluster && ctas * kColWarps * kColKeep < k) ctas *= 2;
+    const int share = ((k + ctas - 1) / ctas + 15) / 16 * 16;            // whole 16-byte words
+    const int64_t blocks = (rows + kColRows - 1) / kColRows * ctas;
+    AFB_CHECK(blocks < (1LL << 31), "too many rows for one launch");
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)blocks, 1, 1);
+    cfg.blockDim = dim3(32 * kColWarps, 1, 1);
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    auto go = [&](auto v) {
+        AFB_CUDA(cudaLaunchKernelEx(&cfg, quantize_columns_kernel<T, decltype(v)::value>, rows, k, share, x, ld_x, norm, q, ld_q, scale));
+    };
+    if (share <= kColWarps * 8) go(std::integral_constant<int, 8>{});
+    else if (share <= kColWarps * 16) go(std::integral_constant<int, 16>{});
+    else if (share <= kColWarps * 24) go(std::integral_constant<int, 24>{});
+    else if (share <= kColWarps * 32) go(std::integral_constant<int, 32>{});
+    else go(std::integral_constant<int, kColKeep>{});
+}
+
 void quantize(int64_t rows, int64_t k, int type, const void *x, int64_t ld_x, int x_trans, const Norm &norm, int8_t *q,
               int64_t ld_q, float *scale, cudaStream_t s) {
     with_type(type, [&](auto t) {
         using T = decltype(t);
         const T *src = static_cast<const T *>(x);
         if (x_trans) {
-            const int64_t blocks = (rows + kColRows - 1) / kColRows * kColCluster;
-            AFB_CHECK(blocks < (1LL << 31), "too many rows for one launch");
-            quantize_columns_kernel<T><<<(unsigned)blocks, 32 * kColWarps, 0, s>>>(rows, k, src, ld_x, norm, q, ld_q, scale);
-        } else {
-            // as few pieces a thread as hold the row wherever it starts
-            auto go = [&](auto p) {
-                quantize_rows_kernel<T, decltype(p)::value><<<(unsigned)rows, kRowThreads, 0, s>>>(k, src, ld_x, norm, q, ld_q, scale);
-            };
-            const int64_t pieces = (k + 16 + kRowThreads * Piece<T>::kPer - 1) / (kRowThreads * Piece<T>::kPer);
-            if (pieces <= 1) go(std::integral_constant<int, 1>{});
-            else if (pieces <= 2) go(std::integral_constant<int, 2>{});
-            else if (pieces <= 3) go(std::integral_constant<int, 3>{});
-            else if (pieces <= 5) go(std::integral_constant<int, 5>{});
-            else go(std::integral_constant<int, kRowPieces>{});
+            quantize_columns<T>(rows, (int)k, src, ld_x, norm, q, ld_q, scale, s);
+            return;
         }
+        // as few pieces a thread as hold the row wherever it starts
+        const int64_t pieces = (k + 16) / Piece<T>::kPer + 1;
+        auto go = [&](auto p) {
+            quantize_rows_kernel<T, decltype(p)::value><<<(unsigned)rows, kRowThreads, 0, s>>>((int)k, src, ld_x, norm, q, ld_q, scale);
+        };
+        if (pieces <= kRowThreads) go(std::integral_constant<int, 1>{});
+        else if (pieces <= 2 * kRowThreads) go(std::integral_constant<int, 2>{});
+        else if (pieces <= 3 * kRowThreads) go(std::integral_constant<int, 3>{});
+        else if (pieces <= 5 * kRowThreads) go(std::integral_constant<int, 5>{});
+        else go(std::integral_constant<int, 8>{});
     });
     AFB_LAUNCHED();
 }

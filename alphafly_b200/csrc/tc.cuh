@@ -81,6 +81,11 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
     return r;
 }
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r));
+    return r;
+}
 __device__ __forceinline__ uint32_t cluster_id() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%clusterid.x;\n" : "=r"(r));
