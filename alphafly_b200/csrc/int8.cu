@@ -95,9 +95,10 @@ struct LargestOf<float> {
 constexpr int kRowThreads = 128;
 
 // One CTA per row of x (element (i, k) at x[i ld + k]), P pieces a thread.  The row is read in 16-byte pieces wherever it
-// starts and, where the CTA's pieces hold it, kept in registers (longer rows are read again, from cache); the quantised
-// bytes are shifted to their place through shared memory and leave as 16-byte words, zero past k.
-template <typename T, int P>
+// starts and kept in registers (kLong: read in spans, twice, the second time from cache); the quantised bytes are shifted
+// to their place through shared memory and leave as 16-byte words, zero past k.  The statistics and the long rows have
+// code of their own: with it in the loops they ran out of the instruction cache (35,840 x 2333 float32: 110 us against X).
+template <typename T, int P, bool kLong, bool kNorm>
 __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int k_dim, const T *__restrict__ x, int64_t ld, Norm norm,
                                                                     int8_t *__restrict__ q, int64_t ld_q, float *__restrict__ scale) {
     constexpr int kPer = Piece<T>::kPer, kSpan = kRowThreads * P * kPer;
@@ -117,17 +118,17 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int k_dim, c
     auto value = [&](int base, int p, int e) {
         const float v = to_float(mine[p].e[e]);
         const int k = first_of(base, p) + e;
-        return norm.mean && k >= 0 && k < k_dim ? norm(v, k) : v;
+        return kNorm && k >= 0 && k < k_dim ? norm(v, k) : v;
     };
     if (threadIdx.x == 0) amax = 0u;
     __syncthreads();
     LargestOf<T> largest;
     unsigned m = 0u;
-    for (int base = 0; base < k_dim; base += kStep) {
+    for (int base = 0; base < (kLong ? k_dim : 1); base += kStep) {
         load(base);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            if (norm.mean) {
+            if (kNorm) {
 #pragma unroll
                 for (int e = 0; e < kPer; ++e) m = max(m, magnitude(value(base, p, e)));
             } else {
@@ -140,8 +141,8 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int k_dim, c
     __syncthreads();
     const float s = row_scale(amax), inv = inverse(s);
     if (threadIdx.x == 0) scale[i] = s;
-    for (int base = 0; base < k_dim; base += kStep) {
-        if (k_dim > kStep) load(base);
+    for (int base = 0; base < (kLong ? k_dim : 1); base += kStep) {
+        if (kLong) load(base);
 #pragma unroll
         for (int p = 0; p < P; ++p)                                      // byte b of the span: element base - lead + b
 #pragma unroll
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int k_dim, c
                 make_uint4(__funnelshift_r(w[0], w[1], by), __funnelshift_r(w[1], w[2], by), __funnelshift_r(w[2], w[3], by),
                            __funnelshift_r(w[3], w[4], by));
         }
-        if (k_dim > kStep) __syncthreads();
+        if (kLong) __syncthreads();
     }
 }
 
@@ -174,7 +175,7 @@ constexpr int kColKeep = 40;                     // most values a thread keeps
 // rows, each CTA a part of k; the CTAs' largest magnitudes meet through distributed shared memory.  Up to 320 values of k
 // a CTA stay in registers, V a thread (beyond 2,560 they are read again, from cache); the bytes are transposed in shared
 // memory.
-template <typename T, int V>
+template <typename T, int V, bool kNorm>
 __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
     quantize_columns_kernel(int64_t rows, int k_dim, int share, const T *__restrict__ x, int64_t ld, Norm norm, int8_t *__restrict__ q,
                             int64_t ld_q, float *__restrict__ scale) {
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
             const int k = base + k_of(p);
             mine[p] = in && k < k1 ? to_float(x[k * ld + i]) : 0.f;
         }
-        if (norm.mean)
+        if (kNorm)
 #pragma unroll
             for (int p = 0; p < V; ++p) {
                 const int k = base + k_of(p);
@@ -643,7 +644,9 @@ void quantize_columns(int64_t rows, int k, const T *x, int64_t ld_x, const Norm 
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     auto go = [&](auto v) {
-        AFB_CUDA(cudaLaunchKernelEx(&cfg, quantize_columns_kernel<T, decltype(v)::value>, rows, k, share, x, ld_x, norm, q, ld_q, scale));
+        constexpr int V = decltype(v)::value;
+        if (norm.mean) AFB_CUDA(cudaLaunchKernelEx(&cfg, quantize_columns_kernel<T, V, true>, rows, k, share, x, ld_x, norm, q, ld_q, scale));
+        else AFB_CUDA(cudaLaunchKernelEx(&cfg, quantize_columns_kernel<T, V, false>, rows, k, share, x, ld_x, norm, q, ld_q, scale));
     };
     if (share <= kColWarps * 8) go(std::integral_constant<int, 8>{});
     else if (share <= kColWarps * 16) go(std::integral_constant<int, 16>{});
@@ -663,14 +666,18 @@ void quantize(int64_t rows, int64_t k, int type, const void *x, int64_t ld_x, in
         }
         // as few pieces a thread as hold the row wherever it starts
         const int64_t pieces = (k + 16) / Piece<T>::kPer + 1;
-        auto go = [&](auto p) {
-            quantize_rows_kernel<T, decltype(p)::value><<<(unsigned)rows, kRowThreads, 0, s>>>((int)k, src, ld_x, norm, q, ld_q, scale);
+        auto go = [&](auto p, auto is_long) {
+            constexpr int P = decltype(p)::value;
+            constexpr bool kLong = decltype(is_long)::value;
+            if (norm.mean) quantize_rows_kernel<T, P, kLong, true><<<(unsigned)rows, kRowThreads, 0, s>>>((int)k, src, ld_x, norm, q, ld_q, scale);
+            else quantize_rows_kernel<T, P, kLong, false><<<(unsigned)rows, kRowThreads, 0, s>>>((int)k, src, ld_x, norm, q, ld_q, scale);
         };
-        if (pieces <= kRowThreads) go(std::integral_constant<int, 1>{});
-        else if (pieces <= 2 * kRowThreads) go(std::integral_constant<int, 2>{});
-        else if (pieces <= 3 * kRowThreads) go(std::integral_constant<int, 3>{});
-        else if (pieces <= 5 * kRowThreads) go(std::integral_constant<int, 5>{});
-        else go(std::integral_constant<int, 8>{});
+        if (pieces <= kRowThreads) go(std::integral_constant<int, 1>{}, std::false_type{});
+        else if (pieces <= 2 * kRowThreads) go(std::integral_constant<int, 2>{}, std::false_type{});
+        else if (pieces <= 3 * kRowThreads) go(std::integral_constant<int, 3>{}, std::false_type{});
+        else if (pieces <= 5 * kRowThreads) go(std::integral_constant<int, 5>{}, std::false_type{});
+        else if (pieces <= 8 * kRowThreads) go(std::integral_constant<int, 8>{}, std::false_type{});
+        else go(std::integral_constant<int, 8>{}, std::true_type{});
     });
     AFB_LAUNCHED();
 }
