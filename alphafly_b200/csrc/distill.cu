@@ -313,9 +313,20 @@ __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restric
     const T *row = logits + i * ld;
     const int lead = lead_of(row), lane = threadIdx.x & 31;
     Piece<T> mine[kChunk];
-    auto load = [&](int at) {                    // the chunk whose first piece starts at `at`
+    // no piece is partly of the row: shorter code for float32 (168 us against 158 at 35,840 x 4168), none for 16-bit types
+    const bool whole = sizeof(T) == 4 && lead == 0 && n_moves % kPer == 0;
+    Piece<T> nothing;
 #pragma unroll
-        for (int p = 0; p < kChunk; ++p) mine[p] = load_piece(row, at + p * NT * kPer, n_moves, from_float<T>(-kInf));
+    for (int e = 0; e < kPer; ++e) nothing.e[e] = from_float<T>(-kInf);
+    auto load = [&](int at) {                    // the chunk whose first piece starts at `at`
+        if (whole) {
+#pragma unroll
+            for (int p = 0; p < kChunk; ++p)
+                mine[p].raw = at + p * NT * kPer < n_moves ? __ldg(reinterpret_cast<const uint4 *>(row + at + p * NT * kPer)) : nothing.raw;
+        } else {
+#pragma unroll
+            for (int p = 0; p < kChunk; ++p) mine[p] = load_piece(row, at + p * NT * kPer, n_moves, from_float<T>(-kInf));
+        }
     };
     const int first = (int)threadIdx.x * kPer - lead, step = kChunk * NT * kPer;
     FourMax<T> max4;
