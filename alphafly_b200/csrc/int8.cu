@@ -188,19 +188,27 @@ __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
     if (threadIdx.x < kColRows) amax[threadIdx.x] = 0u;
     __syncthreads();
     const bool in = i < rows;
+    const T *const column = x + min(i, rows - 1);                        // lanes past the rows read the last one
     float mine[V];
     auto k_of = [&](int p) { return (p / 4 * kColWarps + warp) * 4 + p % 4; };   // a thread's fours are neighbours in k
     auto load = [&](int base) {
 #pragma unroll
-        for (int p = 0; p < V; ++p) {
+        for (int p = 0; p < V; p += 4) {
             const int k = base + k_of(p);
-            mine[p] = in && k < k1 ? to_float(x[k * ld + i]) : 0.f;
+            const T *const at = column + (int64_t)k * ld;
+            if (k + 4 <= k1) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mine[p + j] = to_float(at[j * ld]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mine[p + j] = k + j < k1 ? to_float(at[j * ld]) : 0.f;
+            }
         }
         if (kNorm)
 #pragma unroll
             for (int p = 0; p < V; ++p) {
                 const int k = base + k_of(p);
-                if (in && k < k1) mine[p] = norm(mine[p], k);
+                if (k < k1) mine[p] = norm(mine[p], k);
             }
     };
     unsigned m = 0u;
@@ -219,6 +227,7 @@ __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
         asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(tc::map_to(own, (uint32_t)c)) : "memory");
         m = max(m, v);
     }
+    if (ctas > 1) tc::cluster_arrive_relaxed();  // the maxima are read
     const float s = row_scale(m), inv = inverse(s);
     if (k0 == 0 && warp == 0 && in) scale[i] = s;
     for (int base = k0; base < k1; base += kSpan) {
@@ -233,7 +242,7 @@ __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
         for (int r = warp; r < kColRows && i0 + r < rows; r += kColWarps)
             for (int w = lane; w < words; w += 32) *reinterpret_cast<uint32_t *>(q + (i0 + r) * ld_q + base + 4 * w) = tile[r][w];
     }
-    if (ctas > 1) tc::cluster_sync();            // no CTA ends while another may read its maxima
+    if (ctas > 1) tc::cluster_wait();            // no CTA ends while another may read its maxima
 }
 
 // ---- few rows ------------------------------------------------------------------------------------------------

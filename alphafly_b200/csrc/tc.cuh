@@ -106,6 +106,10 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
+// The two halves of a barrier that orders no memory: every CTA has come here before any leaves the wait.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
+
 // Bounded wait that also gives up as soon as another thread has reported a failure.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const int *status) {
     for (uint32_t it = 0; it < kWaitLimit; ++it) {
