@@ -21,7 +21,6 @@
 namespace afb {
 namespace {
 
-constexpr float kInf = __builtin_huge_valf();
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int kThreads = 128;                   // of a CTA, but 256 for rows too long for its registers
 constexpr int kWarps = 16;                      // at most
@@ -999,35 +998,6 @@ void by_row_length(int64_t n, F &&f) {
     else if (pieces <= 5 * kThreads) f(Few{}, std::integral_constant<int, 5>{});
     else if (pieces <= 9 * kThreads) f(Few{}, std::integral_constant<int, 9>{});
     else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
-}
-
-// Lets the kernel take that much dynamic shared memory on the current device; asked for once per size that is needed.
-template <auto kKernel>
-void allow_shared(size_t bytes) {
-    static size_t allowed[64] = {0};
-    if (bytes <= 32 * 1024) return;
-    int dev = 0;
-    AFB_CUDA(cudaGetDevice(&dev));
-    if (dev < 64 && allowed[dev] >= bytes) return;
-    AFB_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (dev < 64) allowed[dev] = bytes;
-}
-
-// CTAs of a kernel that the current device holds at once (asked for again when the shared memory changes).
-template <auto kKernel>
-int64_t resident(int threads, size_t shared) {
-    static size_t of[64] = {0};
-    static int64_t ctas[64] = {0};
-    int dev = 0;
-    AFB_CUDA(cudaGetDevice(&dev));
-    if (dev < 64 && ctas[dev] && of[dev] == shared) return ctas[dev];
-    int per_sm = 0, sms = 0;
-    AFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, threads, shared));
-    AFB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    AFB_CHECK(per_sm >= 1, "the kernel does not fit on this device");
-    const int64_t n = (int64_t)per_sm * sms;
-    if (dev < 64) of[dev] = shared, ctas[dev] = n;
-    return n;
 }
 
 void check_rows(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k, float temperature,

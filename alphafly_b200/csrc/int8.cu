@@ -7,8 +7,8 @@
 // kMaxK = 2^17 - 1 of them.  A row of zeros has s = 0 and q = 0; a row that holds an infinity or a NaN has
 // s = NaN and q = 0, so its results are NaN and no other row's.
 //
-// Kernels: quantize_rows_kernel and quantize_columns_kernel by the layout of x, dot_kernel for a few rows (quantisation
-// and product in one launch), pair_kernel for the rest, on the tensor cores.  The largest magnitude of a row is an
+// Kernels: quantize_rows_kernel and quantize_columns_kernel by the layout of x, dot_kernel for one row (quantisation and
+// product in one launch), pair_kernel for the rest, on the tensor cores.  The largest magnitude of a row is an
 // integer maximum of the magnitudes' bits, which order like the magnitudes and put NaN on top.
 #include <cstring>
 #include <type_traits>
@@ -97,7 +97,7 @@ constexpr int kRowThreads = 128;
 // One CTA per row of x (element (i, k) at x[i ld + k]), P pieces a thread.  The row is read in 16-byte pieces wherever it
 // starts and kept in registers (kLong: read in spans, twice, the second time from cache); the quantised bytes are shifted
 // to their place through shared memory and leave as 16-byte words, zero past k.  The statistics and the long rows have
-// code of their own: with it in the loops they ran out of the instruction cache (35,840 x 2333 float32: 110 us against X).
+// code of their own: with it in the loops they ran out of the instruction cache (35,840 x 2333 float32: 110 us against 76, 5.5 TB/s).
 template <typename T, int P, bool kLong, bool kNorm>
 __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(int k_dim, const T *__restrict__ x, int64_t ld, Norm norm,
                                                                     int8_t *__restrict__ q, int64_t ld_q, float *__restrict__ scale) {
@@ -245,11 +245,13 @@ __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
     if (ctas > 1) tc::cluster_wait();            // no CTA ends while another may read its maxima
 }
 
-// ---- few rows ------------------------------------------------------------------------------------------------
+// ---- one row -------------------------------------------------------------------------------------------------
 
 constexpr int kDotWarps = 8;
-constexpr int kDotRows = 8;                      // most rows of this path
-constexpr int kAhead = 5;                        // 16-byte words of w a lane fetches before the rows are at hand
+constexpr int kDotThreads = 32 * kDotWarps;
+constexpr int kDotMost = 128 * 1024;             // longest row, in bytes of shared memory
+constexpr int kAhead = 5;                        // 16-byte words of w a lane fetches before the row is at hand
+constexpr int kFours = 4;                        // fours of x a thread keeps: rows up to 4,096
 
 __device__ __forceinline__ int dot16(const uint4 &a, const uint4 &b, int acc) {
     acc = __dp4a((int)a.x, (int)b.x, acc);
@@ -258,91 +260,94 @@ __device__ __forceinline__ int dot16(const uint4 &a, const uint4 &b, int acc) {
     return __dp4a((int)a.w, (int)b.w, acc);
 }
 
-// y = x w^T for up to R rows in one launch: every CTA quantises the rows into shared memory (kFused; else copies them
-// from q) while its first words of w are on the way, then each warp takes one channel.  Bound by latency: w is 9.7 MB
-// at 2333 x 4171, all of it in flight at once.
-template <typename T, typename O, int R, bool kFused>
-__global__ void __launch_bounds__(32 * kDotWarps)
-    dot_kernel(int rows, int64_t n, int k_dim, const T *__restrict__ x, int64_t row_step, int64_t k_step, Norm norm,
-               const float *__restrict__ q_scale, const int8_t *__restrict__ w, int64_t ld_w, const float *__restrict__ w_scale,
-               const float *__restrict__ bias, O *__restrict__ y, int64_t ld_y) {
-    extern __shared__ uint4 held[];              // R rows of `words` 16-byte words, zero past k_dim
-    __shared__ unsigned amax[R];
+// y = x w^T for one row in one launch: every CTA quantises the row into shared memory (kFused; else copies it from q)
+// while its first words of w are on the way, then each of its warps takes a channel at a time.  Bound by latency: two
+// trips to memory and a barrier; w is 9.7 MB at 2333 x 4171, all of it in flight at once.
+template <typename T, typename O, bool kFused>
+__global__ void __launch_bounds__(kDotThreads) dot_kernel(int64_t n, int k_dim, const T *__restrict__ x, int64_t k_step, Norm norm,
+                                                          const float *__restrict__ q_scale, const int8_t *__restrict__ w, int64_t ld_w,
+                                                          const float *__restrict__ w_scale, const float *__restrict__ bias,
+                                                          O *__restrict__ y) {
+    extern __shared__ uint4 held[];              // the row in 16-byte words, zero past k_dim
+    __shared__ unsigned amax;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, words = (k_dim + 15) / 16;
-    const int64_t j = (int64_t)blockIdx.x * kDotWarps + warp;
-    // w's last word may hold anything past k_dim: the rows hold zeros there
-    const uint4 *const wr = reinterpret_cast<const uint4 *>(w + (j < n ? j : 0) * ld_w);
+    const int64_t first = (int64_t)blockIdx.x * kDotWarps + warp, step = (int64_t)gridDim.x * kDotWarps;
+    // w's last word may hold anything past k_dim: the row holds zeros there
+    auto row_of = [&](int64_t j) { return reinterpret_cast<const uint4 *>(w + j * ld_w); };
     uint4 ahead[kAhead];
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) ahead[a] = lane + 32 * a < words ? __ldg(wr + lane + 32 * a) : make_uint4(0u, 0u, 0u, 0u);
-    int8_t *const bytes = reinterpret_cast<int8_t *>(held);
+    for (int a = 0; a < kAhead; ++a)
+        ahead[a] = first < n && lane + 32 * a < words ? __ldg(row_of(first) + lane + 32 * a) : make_uint4(0u, 0u, 0u, 0u);
+    float scale;
     if (kFused) {
-        if (threadIdx.x < R) amax[threadIdx.x] = 0u;
-        __syncthreads();
-        for (int r = 0; r < rows; ++r) {
-            unsigned m = 0u;
-            for (int k = threadIdx.x; k < k_dim; k += 32 * kDotWarps)
-                m = max(m, magnitude(norm(to_float(x[r * row_step + k * k_step]), k)));
-            m = __reduce_max_sync(0xffffffffu, m);
-            if (lane == 0) atomicMax(&amax[r], m);
+        auto value = [&](int k) { return k < k_dim ? norm(to_float(x[k * k_step]), k) : 0.f; };
+        const bool kept = k_dim <= kFours * 4 * kDotThreads;
+        float mine[kFours][4];
+        unsigned m = 0u;
+        if (kept) {
+#pragma unroll
+            for (int f = 0; f < kFours; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mine[f][e] = value((f * kDotThreads + (int)threadIdx.x) * 4 + e);
+#pragma unroll
+            for (int f = 0; f < kFours; ++f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = max(m, magnitude(mine[f][e]));
+        } else {
+            for (int k = threadIdx.x; k < k_dim; k += kDotThreads) m = max(m, magnitude(value(k)));
         }
+        if (threadIdx.x == 0) amax = 0u;
         __syncthreads();
-        for (int r = 0; r < rows; ++r) {
-            const float s = row_scale(amax[r]), inv = inverse(s);
-            auto value = [&](int k) { return k < k_dim ? norm(to_float(x[r * row_step + k * k_step]), k) : 0.f; };
-            for (int k = threadIdx.x * 4; k < words * 16; k += 128 * kDotWarps)
-                *reinterpret_cast<uint32_t *>(bytes + r * words * 16 + k) = quantize4(value(k), value(k + 1), value(k + 2), value(k + 3), s, inv);
+        m = __reduce_max_sync(0xffffffffu, m);
+        if (lane == 0) atomicMax(&amax, m);
+        __syncthreads();
+        scale = row_scale(amax);
+        const float inv = inverse(scale);
+        uint32_t *const fours = reinterpret_cast<uint32_t *>(held);
+        if (kept) {
+#pragma unroll
+            for (int f = 0; f < kFours; ++f) {
+                const int at = f * kDotThreads + (int)threadIdx.x;
+                if (at < words * 4) fours[at] = quantize4(mine[f][0], mine[f][1], mine[f][2], mine[f][3], scale, inv);
+            }
+        } else {
+            for (int at = threadIdx.x; at < words * 4; at += kDotThreads)
+                fours[at] = quantize4(value(at * 4), value(at * 4 + 1), value(at * 4 + 2), value(at * 4 + 3), scale, inv);
         }
     } else {
-        for (int e = threadIdx.x; e < rows * words * 16; e += 32 * kDotWarps) {
-            const int r = e / (words * 16), k = e % (words * 16);
-            bytes[e] = k < k_dim ? (int8_t)x[r * row_step + k] : (int8_t)0;
-        }
+        scale = *q_scale;
+        int8_t *const bytes = reinterpret_cast<int8_t *>(held);
+        for (int k = threadIdx.x; k < words * 16; k += kDotThreads) bytes[k] = k < k_dim ? (int8_t)x[k] : (int8_t)0;
     }
     __syncthreads();
-    if (j >= n) return;
-    int acc[R] = {};
+    for (int64_t j = first; j < n; j += step) {
+        int acc = 0;
+        if (j != first)
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a)
-        if (lane + 32 * a < words)
+            for (int a = 0; a < kAhead; ++a) ahead[a] = lane + 32 * a < words ? __ldg(row_of(j) + lane + 32 * a) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-                if (r < rows) acc[r] = dot16(held[r * words + lane + 32 * a], ahead[a], acc[r]);
-    for (int c = lane + 32 * kAhead; c < words; c += 32) {
-        const uint4 wv = __ldg(wr + c);
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-            if (r < rows) acc[r] = dot16(held[r * words + c], wv, acc[r]);
-    }
-    const float ws = w_scale[j], b = bias ? bias[j] : 0.f;
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        if (r >= rows) break;
-        const int v = __reduce_add_sync(0xffffffffu, acc[r]);
-        const float s = kFused ? row_scale(amax[r]) : q_scale[r];
-        if (lane == r) y[r * ld_y + j] = from_float<O>(fmaf((float)v * ws, s, b));
+        for (int a = 0; a < kAhead; ++a)
+            if (lane + 32 * a < words) acc = dot16(held[lane + 32 * a], ahead[a], acc);
+        for (int c = lane + 32 * kAhead; c < words; c += 32) acc = dot16(held[c], __ldg(row_of(j) + c), acc);
+        acc = __reduce_add_sync(0xffffffffu, acc);
+        if (lane == 0) y[j] = from_float<O>(fmaf((float)acc * w_scale[j], scale, bias ? bias[j] : 0.f));
     }
 }
 
-// At most kDotRows rows, their bytes within the shared memory of a CTA.
-bool few_rows(int64_t rows, int64_t k) { return rows <= kDotRows && rows * ((k + 15) / 16 * 16) <= 96 * 1024; }
+// One row that fits the shared memory of a CTA.  (Two rows are as fast on the tensor cores: 11.8 us at 2333 x 4171, where
+// one row takes 7.2 here, most of it the quantisation that every CTA repeats.)
+bool one_row(int64_t rows, int64_t k) { return rows == 1 && (k + 15) / 16 * 16 <= kDotMost; }
 
 template <typename T, bool kFused>
-void launch_dot(int64_t rows, int64_t n, int64_t k, const T *x, int64_t row_step, int64_t k_step, const Norm &norm,
-                const float *q_scale, const int8_t *w, int64_t ld_w, const float *w_scale, const float *bias, void *y, int y_type,
-                int64_t ld_y, cudaStream_t s) {
-    const size_t shared = (size_t)rows * ((k + 15) / 16 * 16);
+void launch_dot(int64_t n, int64_t k, const T *x, int64_t k_step, const Norm &norm, const float *q_scale, const int8_t *w, int64_t ld_w,
+                const float *w_scale, const float *bias, void *y, int y_type, cudaStream_t s) {
+    const size_t shared = (size_t)((k + 15) / 16 * 16);
     with_type(y_type, [&](auto t) {
         using O = decltype(t);
-        auto go = [&](auto r) {
-            auto kernel = dot_kernel<T, O, decltype(r)::value, kFused>;
-            if (shared > 48 * 1024) AFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared));
-            kernel<<<(unsigned)((n + kDotWarps - 1) / kDotWarps), 32 * kDotWarps, shared, s>>>(
-                (int)rows, n, (int)k, x, row_step, k_step, norm, q_scale, w, ld_w, w_scale, bias, static_cast<O *>(y), ld_y);
-        };
-        if (rows == 1) go(std::integral_constant<int, 1>{});
-        else if (rows <= 4) go(std::integral_constant<int, 4>{});
-        else go(std::integral_constant<int, 8>{});
+        constexpr auto kernel = dot_kernel<T, O, kFused>;
+        allow_shared<kernel>(shared);
+        const int64_t ctas = std::min<int64_t>((n + kDotWarps - 1) / kDotWarps, resident<kernel>(kDotThreads, shared));
+        kernel<<<(unsigned)ctas, kDotThreads, shared, s>>>(n, (int)k, x, k_step, norm, q_scale, w, ld_w, w_scale, bias, static_cast<O *>(y));
     });
     AFB_LAUNCHED();
 }
@@ -693,8 +698,8 @@ void quantize(int64_t rows, int64_t k, int type, const void *x, int64_t ld_x, in
 
 void matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w, int64_t ld_w,
             const float *w_scale, const float *bias, void *y, int y_type, int64_t ld_y, int *status, cudaStream_t s) {
-    if (few_rows(rows, k)) {
-        launch_dot<int8_t, false>(rows, n, k, q, ld_q, 1, Norm{}, q_scale, w, ld_w, w_scale, bias, y, y_type, ld_y, s);
+    if (one_row(rows, k)) {
+        launch_dot<int8_t, false>(n, k, q, 1, Norm{}, q_scale, w, ld_w, w_scale, bias, y, y_type, s);
         return;
     }
     with_type(y_type, [&](auto t) {
@@ -770,7 +775,7 @@ int afb_int8_matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t
 }
 
 size_t afb_int8_linear_workspace(int64_t rows, int64_t k) {
-    if (rows <= 0 || k <= 0 || few_rows(rows, k)) return 0;
+    if (rows <= 0 || k <= 0 || one_row(rows, k)) return 0;
     return align256((size_t)rows * round128(k)) + align256((size_t)rows * 4) + 256;
 }
 
@@ -787,11 +792,11 @@ int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, const void *
         const size_t need = afb_int8_linear_workspace(rows, k);
         AFB_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (afb_int8_linear_workspace)");
         const Norm norm{mean, var, eps, clip};
-        if (few_rows(rows, k)) {
+        if (one_row(rows, k)) {
             with_type(x_type, [&](auto t) {
                 using T = decltype(t);
-                launch_dot<T, true>(rows, n, k, static_cast<const T *>(x), x_trans ? 1 : ld_x, x_trans ? ld_x : 1, norm, nullptr, w,
-                                    ld_w, w_scale, bias, y, y_type, ld_y, as_stream(stream));
+                launch_dot<T, true>(n, k, static_cast<const T *>(x), x_trans ? ld_x : 1, norm, nullptr, w, ld_w, w_scale, bias, y, y_type,
+                                    as_stream(stream));
             });
             return;
         }
