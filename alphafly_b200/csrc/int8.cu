@@ -449,6 +449,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                 if (++s == stages) s = 0, ++use;
             }
         }
+        // after a failure no copy may outlive the CTA: wait, with a limit, for the last of each stage (both CTAs' bytes)
+        if (!ok && rank == 0)
+            for (int d = 0; d < stages; ++d) {
+                const int last = d < s ? use : use - 1;
+                if (last >= 0) tc::bar_wait(full(d), last & 1);
+            }
+        __syncwarp();
     } else if (warp == 1 && rank == 0) {                                 // MMA issuer (leader): the whole warp, so that
         int s = 0, use = 0, ti = 0;                                      // its state is uniform; one lane issues
         bool ok = true;
@@ -569,23 +576,61 @@ void encode_result(CUtensorMap *map, O *y, int64_t rows, int64_t n, int64_t ld) 
     AFB_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (result) failed with code " + std::to_string((int)r));
 }
 
-// Pairs of CTAs that the device holds at once (one CTA per SM).
+// The launch of pairs of CTAs, and how many pairs the current device holds at once (one CTA per SM).
+struct PairLaunch {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    explicit PairLaunch(cudaStream_t s) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.blockDim = dim3(kPairThreads, 1, 1);
+        cfg.dynamicSmemBytes = kPairSmem;
+        cfg.stream = s;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+    }
+};
+
+template <typename O>
 int device_pairs() {
     static int pairs[64] = {0};
     int dev = 0;
     AFB_CUDA(cudaGetDevice(&dev));
     AFB_CHECK(dev >= 0 && dev < 64, "device index out of range");
     if (!pairs[dev]) {
-        int sms = 0;
+        AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+        int sms = 0, n = 0;
         AFB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-        pairs[dev] = sms / 2;
+        PairLaunch launch(nullptr);
+        launch.cfg.gridDim = dim3((unsigned)(sms / 2 * 2), 1, 1);
+        AFB_CUDA(cudaOccupancyMaxActiveClusters(&n, pair_kernel<O>, &launch.cfg));
+        AFB_CHECK(n >= 1, "no pair of CTAs of the 8-bit product fits on this device");
+        pairs[dev] = n;
     }
     return pairs[dev];
 }
 
+// Rows of y per tile: the fewest rounds of tiles times the time of one, which is near proportional to 128 + r: 3.3,
+// 4.2, 5.5 and 6.7 us a round at r = 64, 128, 192 and 256 and k = 2333.  1,120 x 2333 -> 4171 takes 17.0 us with the
+// 160 rows that this gives and 19.3 with 256, which are the best for large products.
+int pick_tile_rows(int64_t rows, int64_t n, int64_t pairs) {
+    const int64_t m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf);
+    int best = kMaxRows;
+    int64_t best_cost = INT64_MAX;
+    for (int r = kMaxRows; r >= kRowStep; r -= kRowStep) {
+        const int64_t cost = (m_tiles * ((rows + r - 1) / r) + pairs - 1) / pairs * (128 + r);
+        if (cost < best_cost) best = r, best_cost = cost;
+    }
+    return best;
+}
+
 template <typename O>
-void launch_pairs(int tile_rows, int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w,
+void launch_pairs(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w,
                   int64_t ld_w, const float *w_scale, const float *bias, O *y, int64_t ld_y, int *status, cudaStream_t s) {
+    const int64_t pairs = device_pairs<O>();
+    const int tile_rows = pick_tile_rows(rows, n, pairs);
     CUtensorMap map_w, map_q, map_y;
     tc::encode_operand_s8(&map_w, w, n, k, ld_w, kHalf);
     tc::encode_operand_s8(&map_q, q, rows, k, ld_q, (uint32_t)tile_rows / 2);
@@ -596,42 +641,10 @@ void launch_pairs(int tile_rows, int64_t rows, int64_t n, int64_t k, const int8_
     else std::memset(&map_y, 0, sizeof(map_y));
     const int64_t total = (n + 2 * kHalf - 1) / (2 * kHalf) * ((rows + tile_rows - 1) / tile_rows);
     AFB_CHECK(total < (1LL << 31), "too many rows for one launch");
-    const int64_t pairs = std::min<int64_t>(total, device_pairs());
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
-    cfg.blockDim = dim3(kPairThreads, 1, 1);
-    cfg.dynamicSmemBytes = kPairSmem;
-    cfg.stream = s;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    static bool configured[64] = {false};
-    int dev = 0;
-    AFB_CUDA(cudaGetDevice(&dev));
-    if (dev >= 64 || !configured[dev]) {
-        AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
-        if (dev < 64) configured[dev] = true;
-    }
-    AFB_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<O>, map_w, map_q, map_y, tile_rows, (int)rows, (int)n, (int)k, q_scale, w_scale,
+    PairLaunch launch(s);
+    launch.cfg.gridDim = dim3((unsigned)(2 * std::min(total, pairs)), 1, 1);
+    AFB_CUDA(cudaLaunchKernelEx(&launch.cfg, pair_kernel<O>, map_w, map_q, map_y, tile_rows, (int)rows, (int)n, (int)k, q_scale, w_scale,
                                 bias, y, ld_y, n_tma, status));
-}
-
-// Rows of y per tile: the fewest rounds of tiles times the time of one, which is near proportional to 128 + r: 3.3,
-// 4.2, 5.5 and 6.7 us a round at r = 64, 128, 192 and 256 and k = 2333.  1,120 x 2333 -> 4171 takes 17.0 us with the
-// 160 rows that this gives and 19.3 with 256, which are the best for large products.
-int pick_tile_rows(int64_t rows, int64_t n) {
-    const int64_t m_tiles = (n + 2 * kHalf - 1) / (2 * kHalf), pairs = device_pairs();
-    int best = kMaxRows;
-    int64_t best_cost = INT64_MAX;
-    for (int r = kMaxRows; r >= kRowStep; r -= kRowStep) {
-        const int64_t cost = (m_tiles * ((rows + r - 1) / r) + pairs - 1) / pairs * (128 + r);
-        if (cost < best_cost) best = r, best_cost = cost;
-    }
-    return best;
 }
 
 void check_rows16(const void *p, int64_t ld, const char *what) {
@@ -704,8 +717,7 @@ void matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, c
     }
     with_type(y_type, [&](auto t) {
         using O = decltype(t);
-        launch_pairs<O>(pick_tile_rows(rows, n), rows, n, k, q, ld_q, q_scale, w, ld_w, w_scale, bias, static_cast<O *>(y), ld_y,
-                        status, s);
+        launch_pairs<O>(rows, n, k, q, ld_q, q_scale, w, ld_w, w_scale, bias, static_cast<O *>(y), ld_y, status, s);
     });
 }
 
@@ -731,6 +743,7 @@ void check_product(int64_t n, int64_t k, const void *w, int64_t ld_w, const floa
     AFB_CHECK(known_type(y_type), "unknown element type");
     AFB_CHECK(w && w_scale && y, "NULL pointer");
     AFB_CHECK(ld_w >= k && ld_y >= n, "a leading dimension is below the row length");
+    AFB_CHECK(reinterpret_cast<uintptr_t>(y) % type_size(y_type) == 0, "y is not aligned to its elements");
     check_rows16(w, ld_w, "w");
 }
 
