@@ -1091,8 +1091,13 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
                 allow_shared<kernel>(shared);
                 kernel<<<(unsigned)std::min<int64_t>(rows, resident<kernel>(NT, shared)), NT, shared, s>>>(a, rows, (int)held, x, g);
             };
-            if (held <= 20 * 1024) go(std::integral_constant<int, 128>{}, std::true_type{});
-            else if (held <= 36 * 1024) go(std::integral_constant<int, 256>{}, std::true_type{});
+            // few threads a row, since what every warp does once a row costs more than its share of the elements (35,840 x 4168
+            // float32, 16.7 KB: 205 us with 128 threads, 333 with 256, 768 with 512; 16,000 x 4168 bfloat16 97 us with 128, 83
+            // with 64); the next row on its way where several CTAs fit an SM all the same (4,096 x 16000 bfloat16, 32 KB: 70 us
+            // with it, 61 without and twice the CTAs)
+            if (held <= 10 * 1024) go(std::integral_constant<int, 64>{}, std::true_type{});
+            else if (held <= 20 * 1024) go(std::integral_constant<int, 128>{}, std::true_type{});
+            else if (held <= 40 * 1024) go(std::integral_constant<int, 128>{}, std::false_type{});
             else if (held + more <= 112 * 1024) go(std::integral_constant<int, 256>{}, std::false_type{});
             else {
                 const size_t shared = more;
