@@ -1,17 +1,19 @@
 // Distillation from a teacher's best moves: their selection, and the loss of a student against them with its
 // gradient.
 //
-// top_kernel: for each row of logits l over a support (all moves, or the row's listed moves) the k largest, ties to
-//   the lowest move, and  log_rest = log sum exp(l / T)  over the support's moves that are not among them.  NaN and
-//   -inf are outside the support.  One CTA per row.  A lower bound of the k-th largest comes from the largest value
-//   of each of kGroups groups of moves (k different moves are at least the k-th largest of those); the moves at or
-//   above the bound are collected and ranked by counting.
-// loss_kernel: with p the teacher's distribution over its named moves C (softmax of t / T; with `rest` one more
-//   outcome, any other move, at exp(log_rest)) and q = softmax(s / T) of the student over its support,
+// Selection (top_kernel, top_listed_kernel): for each row of logits l over a support (all moves, or the row's listed
+//   moves) the k largest, ties to the lowest move, and  log_rest = log sum exp(l / T)  over the support's moves that are
+//   not among them.  NaN and -inf are outside the support.  A lower bound of the k-th largest comes from the largest
+//   value of each of 128 to 512 groups of moves (k different moves are at least the k-th largest of those); the few moves
+//   at or above the bound are collected and ranked by counting, the others' exponentials summed in the same pass.
+// Loss (loss_kernel, loss_listed_kernel, loss_long_kernel): with p the teacher's distribution over its named moves C
+//   (softmax of t / T; with `rest` one more outcome, any other move, at exp(log_rest)) and q = softmax(s / T) of the
+//   student over its support,
 //       loss = T^2 sum_c p_c (log p_c - log q_c)                          q_rest = the sum of q outside C
 //       dloss / ds_j = T (q_j - p_j)  in C,   T q_j (1 - p_rest / q_rest)  outside C,  0 outside the support.
-//   The shares of C and of the rest come from the log odds d = lse(C) - lse(rest) as log share(rest) =
-//   -log(1 + exp(d)), so that neither the loss nor the gradient takes a difference of nearly equal sums.
+//   The sums over C and over the rest are taken apart (the rest is not a total less C), so neither the shares nor the
+//   gradient take a difference of nearly equal sums.
+// All sums and exponentials are float32; a gradient is rounded to the logits' type once, scaled.
 #include <cfloat>
 #include <cmath>
 #include <type_traits>
@@ -22,7 +24,7 @@ namespace afb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kThreads = 128;                   // of a CTA, but 256 for rows too long for its registers
+constexpr int kThreads = 128;                   // of a CTA, where nothing else is said
 constexpr int kWarps = 16;                      // at most
 constexpr int kListThreads = 64;                // of a CTA that takes the loss over a row's list (16,000 x 64: 71 us, 109 with 128)
 constexpr int kLongThreads = 256;               // for rows that a CTA does not hold
@@ -248,7 +250,8 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
     if (threadIdx.x == 0) *log_rest = m > -kInf && m < kInf ? m * inv_t + logf(sum) : m;
 }
 
-// The rows' listed moves: all entries are at hand in shared memory.
+// The rows' listed moves: all entries are at hand in shared memory.  Latency of the list, then of the gather (a 32-byte
+// sector a move): 1,120 rows of 64, k = 8: 8.4 us; 35,840 of them 107 us; 35,840 of 218, k = 32: 171 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) top_listed_kernel(int64_t n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
                                                               const int64_t *__restrict__ list, const uint8_t *__restrict__ valid,
@@ -302,7 +305,9 @@ struct FourMax<float> {
 
 // All moves of a row: one CTA per row, of NT threads, P pieces a thread in registers (P = 0: any length, the row is read
 // twice, the second time from cache).  One pass takes the groups' maxima, one collects the moves at or above the bound
-// and sums the exponentials of the others relative to it; one warp ranks the candidates.
+// and sums the exponentials of the others relative to it; one warp ranks the candidates.  35,840 x 4168 float32: 113 us
+// for k = 1 (5.3 TB/s), 159 for 32, 405 for 128; 2,048 x 32000 bfloat16, k = 64: 57 us.  Bound by what a row costs beside
+// its elements: the search for the bound and the ranking are one warp's, while the other CTAs of the SM load.
 template <typename T, int NT, int P>
 __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
                                                  float *__restrict__ values, int64_t *__restrict__ moves,
@@ -339,9 +344,10 @@ __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restric
     float best[4];
 #pragma unroll
     for (int h = 0; h < 4; ++h) best[h] = max4.get(h);
-    // up to four groups a thread, as many as give k of them a good bound
+    // one to four groups a thread, as many as give k of them a good bound
     const float most = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-    if (4 * k <= NT) {
+    const bool one = 4 * k <= NT || NT == kGroups;
+    if (one) {
         sh.group[threadIdx.x] = order_of(most);
     } else if (2 * k <= NT || kGroups == 2 * NT) {
         sh.group[threadIdx.x] = order_of(fmaxf(best[0], best[2]));
@@ -354,8 +360,10 @@ __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restric
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
     if (threadIdx.x < 32) {
-        const unsigned t = 4 * k <= NT ? kth_of_groups<NT>(sh.group, k)
-                           : 2 * k <= NT || kGroups == 2 * NT ? kth_of_groups<2 * NT>(sh.group, k) : kth_of_groups<kGroups>(sh.group, k);
+        const unsigned t = one ? kth_of_groups<NT>(sh.group, k)
+                           : 2 * k <= NT || kGroups == 2 * NT
+                               ? kth_of_groups<(2 * NT < kGroups ? 2 * NT : kGroups)>(sh.group, k)
+                               : kth_of_groups<kGroups>(sh.group, k);
         // at least the lowest finite value, so that -inf stays below it
         if (lane == 0) sh.bound = max(t, order_of(-FLT_MAX));
     }
@@ -641,7 +649,8 @@ __device__ __forceinline__ void write_named(const Named &nm, int k, float odds, 
             g[nm.move[e]] = from_float<T>(some ? f * (expf(log_q_of(nm, e, log_q_named_of(nm, odds), inv_t)) - nm.p[e]) : 0.f);
 }
 
-// Over a row's listed moves: one CTA per row, the lists and their logits in shared memory.
+// Over a row's listed moves: one CTA per row, the lists and their logits in shared memory.  The gradient's zeros are most of
+// the traffic (16,000 x 4168 float32 with 64 listed: 75 us, 3.5 TB/s of zeros); the rest is the latency of list, gather and sums.
 template <typename T>
 __global__ void __launch_bounds__(kListThreads, 20) loss_listed_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits, T *__restrict__ grad) {
     extern __shared__ unsigned dynamic[];
@@ -739,7 +748,9 @@ __device__ __forceinline__ void fetch_row(T *held, const T *row, int n) {
 // (into a second buffer) while it works on one, so that only shared memory is waited for.  The named moves are taken out
 // of the row (-inf), so that its sum is the rest's.  The terms are relative to the teacher's best move: no maximum is
 // taken, one barrier joins the sums.  Sums outside kSmall .. kLarge (logits 69 T from that move's, no such move, NaN,
-// values whose product with 1 / T overflows) are taken again, after subtracting the largest.
+// values whose product with 1 / T overflows) are taken again, after subtracting the largest.  35,840 x 4168 float32: 203
+// us with the gradient (5.9 TB/s of reads and writes), 144 without; 4,096 x 32000 bfloat16 with it 113 us (4.6 TB/s), where
+// the exponentials, each taken twice, fill half of their pipe's time.
 constexpr float kSmall = 1e-30f, kLarge = 1e30f;
 
 template <typename T, int NT, bool kAhead>
@@ -873,7 +884,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) loss_kernel(LossArgs a, int64_t 
     }
 }
 
-// Rows too long for shared memory: read twice, the second time from cache.  As above, but for the marks: no row is held.
+// Rows too long for shared memory: read twice, the second time from cache (2,048 x 32000 float32 with the gradient: 132 us).
 template <typename T>
 __global__ void __launch_bounds__(kLongThreads) loss_long_kernel(LossArgs a, int64_t rows, const T *__restrict__ logits, T *__restrict__ grad) {
     constexpr int kPer = Piece<T>::kPer, kChunk = 4;
@@ -992,7 +1003,9 @@ __global__ void __launch_bounds__(1024) sum_kernel(int64_t rows, const float *__
 }
 
 // Threads of a CTA and 16-byte pieces a thread for rows of n elements: as few as hold a row wherever it starts (few
-// threads: many rows at once); 256 and 0, no row in registers, beyond 4,605 float32 or 9,209 16-bit elements.
+// threads: many rows at once); 0, no row in registers, beyond 4,605 float32 or 9,209 16-bit elements.  There the threads
+// grow with the row: 8,192 x 5000 float32 53 us with 128 threads, 62 with 256; 2,048 x 32000 bfloat16 64, 57 and 62 with
+// 128, 256 and 512; 2,048 x 32000 float32 104, 96 and 78.
 template <typename T, typename F>
 void by_row_length(int64_t n, F &&f) {
     const int64_t pieces = (n + 2 * Piece<T>::kPer - 2) / Piece<T>::kPer;
@@ -1001,7 +1014,9 @@ void by_row_length(int64_t n, F &&f) {
     else if (pieces <= 3 * kThreads) f(Few{}, std::integral_constant<int, 3>{});
     else if (pieces <= 5 * kThreads) f(Few{}, std::integral_constant<int, 5>{});
     else if (pieces <= 9 * kThreads) f(Few{}, std::integral_constant<int, 9>{});
-    else f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
+    else if (pieces <= 20 * kThreads) f(Few{}, std::integral_constant<int, 0>{});
+    else if (pieces <= 24 * 256) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 0>{});
+    else f(std::integral_constant<int, 512>{}, std::integral_constant<int, 0>{});
 }
 
 void check_rows(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k, float temperature,

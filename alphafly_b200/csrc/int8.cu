@@ -375,7 +375,14 @@ __device__ __forceinline__ void mma_pair_s8(uint32_t d_tmem, uint64_t a_desc, ui
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
 
-// Tiles of 2 kHalf channels (MMA M) x tile_rows rows of y (MMA N).
+// y in tiles of 2 kHalf channels (MMA M) x tile_rows rows (MMA N), each a pair of CTAs' (cluster of two, two-SM MMA, M 256,
+// K 32): the pipeline of the float16 input map, in 8 bits.  CTA r of a pair holds channels 128 r .. + 127 and half of the
+// rows of every k block; per block an SM loads 16 KB of w and up to 16 KB of q for 4 MMAs of 128 cycles.  Channels lie
+// along the TMEM lanes, so a row's results are one line.  Two accumulators alternate: the epilogue of a tile (16 warps:
+// int32 to float32, scales, bias, one rounding) runs under the products of the next.  Persistent, channels fastest, so
+// concurrent pairs share rows.  Bound by the tensor pipe in large products: 35,840 x 2333 -> 4171 in 215 us, 3,240 TOP/s
+// (0.96 of twice the measured bf16 rate); by the store of y where k is short: 2,048 x 838 -> 17937 in 34 us, 2.2 TB/s.
+// Every wait is bounded and gives up once the status word is set; TMEM is always released.
 template <typename O>
 __global__ void __launch_bounds__(kPairThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_q,
