@@ -276,7 +276,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-constexpr int kRanked = 96;                      // candidates that one warp ranks by itself
+// Candidates that one warp ranks by itself where many rows keep the SM busy (35,840 x 4168 float32, k = 128: 363 us, 406 with
+// the whole CTA; a single row of k = 64: 6.7 us and 6.0).
+constexpr int kRanked = 160, kManyRows = 1024;
 
 // The largest of each of four subsets of a thread's moves (a maximum passes NaN over); 16-bit types two at a time.
 template <typename T>
@@ -306,7 +308,7 @@ struct FourMax<float> {
 // All moves of a row: one CTA per row, of NT threads, P pieces a thread in registers (P = 0: any length, the row is read
 // twice, the second time from cache).  One pass takes the groups' maxima, one collects the moves at or above the bound
 // and sums the exponentials of the others relative to it; one warp ranks the candidates.  35,840 x 4168 float32: 113 us
-// for k = 1 (5.3 TB/s), 159 for 32, 405 for 128; 2,048 x 32000 bfloat16, k = 64: 57 us.  Bound by what a row costs beside
+// for k = 1 (5.3 TB/s), 159 for 32, 363 for 128; 2,048 x 32000 bfloat16, k = 64: 57 us.  Bound by what a row costs beside
 // its elements: the search for the bound and the ranking are one warp's, while the other CTAs of the SM load.
 template <typename T, int NT, int P>
 __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
@@ -474,14 +476,18 @@ __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restric
     };
     auto in_block = [&](float x, float unit, auto &&f) { return block_reduce(x, sh.scratch, unit, f); };
     auto in_warp = [&](float x, float, auto &&f) { return warp_reduce(x, f); };
-    if (found > kRanked) {
-        if (found <= NT) close((int)threadIdx.x, NT, std::integral_constant<int, 1>{}, in_block);
-        else if (found <= 2 * NT) close((int)threadIdx.x, NT, std::integral_constant<int, 2>{}, in_block);
-        else close((int)threadIdx.x, NT, std::integral_constant<int, kCandidates / NT>{}, in_block);
+    using std::integral_constant;
+    if (found > (gridDim.x >= kManyRows ? kRanked : 32)) {
+        if (found <= NT) close((int)threadIdx.x, NT, integral_constant<int, 1>{}, in_block);
+        else if (found <= 2 * NT) close((int)threadIdx.x, NT, integral_constant<int, 2>{}, in_block);
+        else if (4 * NT < kCandidates && found <= 3 * NT) close((int)threadIdx.x, NT, integral_constant<int, 3>{}, in_block);
+        else if (4 * NT < kCandidates && found <= 4 * NT) close((int)threadIdx.x, NT, integral_constant<int, 4>{}, in_block);
+        else close((int)threadIdx.x, NT, integral_constant<int, kCandidates / NT>{}, in_block);
     } else if (threadIdx.x < 32) {
-        if (found <= 32) close(lane, 32, std::integral_constant<int, 1>{}, in_warp);
-        else if (found <= 64) close(lane, 32, std::integral_constant<int, 2>{}, in_warp);
-        else close(lane, 32, std::integral_constant<int, kRanked / 32>{}, in_warp);
+        if (found <= 32) close(lane, 32, integral_constant<int, 1>{}, in_warp);
+        else if (found <= 64) close(lane, 32, integral_constant<int, 2>{}, in_warp);
+        else if (found <= 96) close(lane, 32, integral_constant<int, 3>{}, in_warp);
+        else close(lane, 32, integral_constant<int, kRanked / 32>{}, in_warp);
     }
 }
 

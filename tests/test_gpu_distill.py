@@ -80,6 +80,20 @@ def test_top_logits_over_sizes(v, k, dtype):
     _check_top((_rand(5, v, seed=v + k) * 2).to(dtype), k, 1.7)
 
 
+@pytest.mark.parametrize("v", [600, 5003])
+@pytest.mark.parametrize("k", [16, 48, 80, 128, 190])
+def test_top_logits_of_many_rows(v, k):
+    """More than 1,024 rows are ranked by one warp each up to 160 candidates; half of the rows have equal values."""
+    x = _rand(1100, v, seed=v + k) * 2
+    x[::2] = (x[::2] * 4).round() / 4
+    _check_top(x, k, 0.8)
+
+
+@pytest.mark.parametrize("k", [100, 170, 256])
+def test_top_logits_of_large_k(k):
+    _check_top(_rand(40, 4168, seed=k), k)
+
+
 @pytest.mark.parametrize("listed", [1, 30, 218, 1500, 4096])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_top_logits_of_legal_moves(listed, dtype):
