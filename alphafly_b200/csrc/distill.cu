@@ -147,33 +147,40 @@ __device__ unsigned kth_of_groups(const unsigned *group, int k) {
     return t;
 }
 
+// Entries that are ranked without a bound: 35,840 lists of 64, k = 8: 92 us, 107 with it; of 100: 151 us, 137 with it.
+constexpr int kFew = 64;
+
 // Selects from `n` entries, get(e, order, move).  A row with too many entries at the bound (many equal values) finds
 // the k-th key itself bit by bit.
 template <int NT, typename Get>
 __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, float *values, int64_t *moves, float *log_rest) {
-    for (int g = threadIdx.x; g < kGroups; g += NT) sh.group[g] = 0u;
     if (threadIdx.x == 0) sh.count = 0;
-    // entry e belongs to group e mod kGroups
-    unsigned best[kGroups / NT] = {};
-    for (int e0 = 0; e0 < n; e0 += kGroups)
+    unsigned bound = 1u;                         // 0: no move
+    if (n > kFew) {
+        // entry e belongs to group e mod kGroups
+        unsigned best[kGroups / NT] = {};
+        for (int e0 = 0; e0 < n; e0 += kGroups)
 #pragma unroll
-        for (int h = 0; h < kGroups / NT; ++h) {
-            const int e = e0 + h * NT + (int)threadIdx.x;
-            if (e >= n) break;
-            unsigned o;
-            int m;
-            get(e, o, m);
-            best[h] = max(best[h], o);
+            for (int h = 0; h < kGroups / NT; ++h) {
+                const int e = e0 + h * NT + (int)threadIdx.x;
+                if (e >= n) break;
+                unsigned o;
+                int m;
+                get(e, o, m);
+                best[h] = max(best[h], o);
+            }
+#pragma unroll
+        for (int h = 0; h < kGroups / NT; ++h) sh.group[h * NT + threadIdx.x] = best[h];
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            const unsigned t = kth_of_groups<kGroups>(sh.group, k);
+            if (threadIdx.x == 0) sh.bound = max(t, 1u);                  // fewer than k groups hold a move
         }
-#pragma unroll
-    for (int h = 0; h < kGroups / NT; ++h) sh.group[h * NT + threadIdx.x] = best[h];
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        const unsigned t = kth_of_groups<kGroups>(sh.group, k);
-        if (threadIdx.x == 0) sh.bound = max(t, 1u);                      // 0: fewer than k groups hold a move
+        __syncthreads();
+        bound = sh.bound;
+    } else {
+        __syncthreads();
     }
-    __syncthreads();
-    unsigned bound = sh.bound;
     for (int e = threadIdx.x; e < n; e += NT) {
         unsigned o;
         int m;
@@ -251,7 +258,7 @@ __device__ void select_top(TopShared &sh, int n, int k, float inv_t, Get &&get, 
 }
 
 // The rows' listed moves: all entries are at hand in shared memory.  Latency of the list, then of the gather (a 32-byte
-// sector a move): 1,120 rows of 64, k = 8: 8.4 us; 35,840 of them 107 us; 35,840 of 218, k = 32: 171 us.
+// sector a move): 1,120 rows of 64, k = 8: 7.4 us; 35,840 of them 92 us; 35,840 of 218, k = 32: 205 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) top_listed_kernel(int64_t n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
                                                               const int64_t *__restrict__ list, const uint8_t *__restrict__ valid,
