@@ -284,8 +284,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // Candidates that one warp ranks by itself where many rows keep the SM busy (35,840 x 4168 float32, k = 128: 363 us, 406 with
-// the whole CTA; a single row of k = 64: 6.7 us and 6.0).
-constexpr int kRanked = 160, kManyRows = 1024;
+// the whole CTA; a single row of k = 64: 6.7 us and 6.0), fewer in larger CTAs (2,048 x 32000 bfloat16, k = 64: 57 and 59 us with
+// 96 and 160).
+constexpr int kRanked = 160, kManyRows = 256;
 
 // The largest of each of four subsets of a thread's moves (a maximum passes NaN over); 16-bit types two at a time.
 template <typename T>
@@ -484,7 +485,8 @@ __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restric
     auto in_block = [&](float x, float unit, auto &&f) { return block_reduce(x, sh.scratch, unit, f); };
     auto in_warp = [&](float x, float, auto &&f) { return warp_reduce(x, f); };
     using std::integral_constant;
-    if (found > (gridDim.x >= kManyRows ? kRanked : 32)) {
+    constexpr int kAlone = NT == kThreads ? kRanked : 96;
+    if (found > (gridDim.x >= kManyRows ? kAlone : 32)) {
         if (found <= NT) close((int)threadIdx.x, NT, integral_constant<int, 1>{}, in_block);
         else if (found <= 2 * NT) close((int)threadIdx.x, NT, integral_constant<int, 2>{}, in_block);
         else if (4 * NT < kCandidates && found <= 3 * NT) close((int)threadIdx.x, NT, integral_constant<int, 3>{}, in_block);
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restric
         if (found <= 32) close(lane, 32, integral_constant<int, 1>{}, in_warp);
         else if (found <= 64) close(lane, 32, integral_constant<int, 2>{}, in_warp);
         else if (found <= 96) close(lane, 32, integral_constant<int, 3>{}, in_warp);
-        else close(lane, 32, integral_constant<int, kRanked / 32>{}, in_warp);
+        else close(lane, 32, integral_constant<int, kAlone / 32>{}, in_warp);
     }
 }
 
