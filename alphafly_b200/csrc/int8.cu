@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
         asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(tc::map_to(own, (uint32_t)c)) : "memory");
         m = max(m, v);
     }
-    if (ctas > 1) tc::cluster_arrive_relaxed();  // the maxima are read
+    if (ctas > 1) tc::cluster_arrive();          // the maxima are read
     const float s = row_scale(m), inv = inverse(s);
     if (k0 == 0 && warp == 0 && in) scale[i] = s;
     for (int base = k0; base < k1; base += kSpan) {
@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(32 * kColWarps, V > 24 ? 3 : 4)
         for (int r = warp; r < kColRows && i0 + r < rows; r += kColWarps)
             for (int w = lane; w < words; w += 32) *reinterpret_cast<uint32_t *>(q + (i0 + r) * ld_q + base + 4 * w) = tile[r][w];
     }
+    __syncwarp();
     if (ctas > 1) tc::cluster_wait();            // no CTA ends while another may read its maxima
 }
 

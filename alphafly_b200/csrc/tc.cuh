@@ -106,9 +106,10 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
 
-// The two halves of a barrier that orders no memory: every CTA has come here before any leaves the wait.
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;\n" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
+// The two halves of cluster_sync: what a CTA read or wrote before it arrived is done when any CTA leaves the wait.  (A relaxed
+// arrival would not do where the barrier keeps shared memory alive for its readers: their loads could still be on the way.)
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;\n" ::: "memory"); }
 
 // Bounded wait that also gives up as soon as another thread has reported a failure.
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const int *status) {
