@@ -1091,6 +1091,7 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
     return guarded([&] {
         check_rows(rows, n_moves, type, logits, ld, k, temperature, legal, valid, n_listed);
         AFB_CHECK(upstream_step >= 0, "negative size");
+        AFB_CHECK(upstream || !skip_ones, "skip_ones needs the upstream gradient");
         if (rows == 0) {
             if (loss) AFB_CUDA(cudaMemsetAsync(loss, 0, 4, as_stream(stream)));
             return;

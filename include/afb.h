@@ -287,8 +287,9 @@ AFB_API int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, cons
  *   has loss and gradient 0.
  *   weight (rows) or NULL (1).  loss (1 float): scale * sum of row_loss.  grad (type, row stride ld_grad):
  *   scale * upstream[i * upstream_step] * the gradient of row_loss[i] by the row's logits, rounded once
- *   (upstream NULL: 1).  With skip_ones the rows whose upstream gradient is 1 are left untouched, for a
- *   gradient that an earlier call wrote.  row_loss, loss, grad may each be NULL (loss needs row_loss).
+ *   (upstream NULL: 1).  With skip_ones (which needs upstream) the rows whose upstream gradient is 1 are left
+ *   untouched, for a gradient that an earlier call wrote.  row_loss, loss, grad may each be NULL (loss needs
+ *   row_loss).
  * Both asynchronous on `stream`; the same inputs give the same bits. */
 AFB_API int afb_top_logits(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k,
                            float temperature, const int64_t *legal, const uint8_t *valid, int64_t n_listed,
