@@ -61,8 +61,11 @@ def _legal(legal, logits: torch.Tensor):
     if moves.dim() != 2:
         raise ValueError(f"legal moves must be (B, K), got {tuple(moves.shape)}")
     shape = (logits.shape[0], moves.shape[1])
-    return (_matrix(moves, shape, torch.int64, logits.device, "legal moves"),
-            _matrix(valid, shape, torch.bool, logits.device, "legal valid"), shape[1])
+    moves = _matrix(moves, shape, torch.int64, logits.device, "legal moves")
+    valid = _matrix(valid, shape, torch.bool, logits.device, "legal valid")
+    if shape[1] == 0:                            # no entries have no address, and no address means all moves
+        moves, valid = moves.new_zeros(shape[0], 1), valid.new_zeros(shape[0], 1)
+    return moves, valid, moves.shape[1]
 
 
 def _ptr(t: torch.Tensor | None):
