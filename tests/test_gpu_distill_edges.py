@@ -29,3 +29,19 @@ def test_lists_of_no_width_hold_no_move(dtype):
         losses = distillation_loss(leaf, named, legal=empty, rest=rest, reduction="none")
         grad, = torch.autograd.grad(losses.sum(), leaf)
         assert not losses.any() and not grad.any()
+
+
+def test_one_row_of_any_stride():
+    """A transposed column is a row whose stride, 1, lies below its length."""
+    column = _rand(300, 1, seed=2)
+    x, plain = column.T, column.reshape(1, 300).clone()
+    assert x.stride() == (1, 1)
+    top, ref = top_logits(x, 6), top_logits(plain, 6)
+    for a, b in zip(top[:3], ref[:3]):
+        assert torch.equal(a, b)
+    leaf, leaf2 = column.clone().requires_grad_(True), plain.clone().requires_grad_(True)
+    for scale in (1.0, 3.0):                     # the forward's gradient, and the backward's
+        loss, loss2 = distillation_loss(leaf.T, top, rest=True), distillation_loss(leaf2, top, rest=True)
+        assert torch.equal(loss, loss2)
+        g, g2 = torch.autograd.grad(loss * scale, leaf)[0], torch.autograd.grad(loss2 * scale, leaf2)[0]
+        assert torch.equal(g.T, g2)
