@@ -290,7 +290,8 @@ AFB_API int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, cons
  *   (upstream NULL: 1).  With skip_ones (which needs upstream) the rows whose upstream gradient is 1 are left
  *   untouched, for a gradient that an earlier call wrote.  row_loss, loss, grad may each be NULL (loss needs
  *   row_loss).
- * Both asynchronous on `stream`; the same inputs give the same bits. */
+ * Both asynchronous on `stream`.  The same inputs give the same bits; a row's sums are taken in an order that goes by
+ * its place on 16 bytes and the number of rows, so elsewhere they may differ in the last ones. */
 AFB_API int afb_top_logits(int64_t rows, int64_t n_moves, int type, const void *logits, int64_t ld, int k,
                            float temperature, const int64_t *legal, const uint8_t *valid, int64_t n_listed,
                            float *values, int64_t *moves, float *log_rest, void *stream);

@@ -45,3 +45,15 @@ def test_one_row_of_any_stride():
         assert torch.equal(loss, loss2)
         g, g2 = torch.autograd.grad(loss * scale, leaf)[0], torch.autograd.grad(loss2 * scale, leaf2)[0]
         assert torch.equal(g.T, g2)
+
+
+@pytest.mark.parametrize("rows,v,k,dtype", [(2048, 4168, 32, torch.float32), (2048, 4168, 128, torch.float32), (64, 4168, 100, torch.float32),
+                                            (1000, 32000, 64, torch.bfloat16), (1000, 12000, 200, torch.float16)])
+def test_selection_repeats_bit_for_bit(rows, v, k, dtype):
+    """Candidates are collected in any order; what is summed of them is not."""
+    x = (_rand(rows, v, seed=k) * 2).to(dtype)
+    first = top_logits(x, k, 2.0)
+    for _ in range(30):
+        again = top_logits(x, k, 2.0)
+        for a, b in zip(first[:3], again[:3]):
+            assert torch.equal(a, b)
