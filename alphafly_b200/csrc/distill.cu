@@ -553,7 +553,8 @@ struct FirstNamed {
 
 // Reads row i's named moves and marks them (all threads; the marks are complete after the return).  keeps(move): whether
 // the student's support has it; value(move): the student's logit; mark(move): sets its mark, whether it was set already.
-template <typename T, typename Keeps, typename Value, typename Mark>
+// kOneMap: marks change what keeps() reads, so every move is asked for first.
+template <bool kOneMap, typename T, typename Keeps, typename Value, typename Mark>
 __device__ __forceinline__ void read_named(const Named &nm, const LossArgs &a, int64_t i, const T *row, const FirstNamed &first,
                                            Keeps &&keeps, Value &&value, Mark &&mark) {
     int again = 0;
@@ -565,7 +566,12 @@ __device__ __forceinline__ void read_named(const Named &nm, const LossArgs &a, i
         nm.move[c] = keep ? (int)m : -1;
         nm.z[c] = t;
         nm.s[c] = keep ? value((int)m) : -kInf;
-        if (keep) again |= mark((int)m);
+        if (!kOneMap && keep) again |= mark((int)m);
+    }
+    if (kOneMap) {
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.k; c += blockDim.x)
+            if (nm.move[c] >= 0) again |= mark(nm.move[c]);
     }
     if (__syncthreads_or(again)) {              // rare: a move named twice counts at its first place
         for (int c0 = 0; c0 < a.k; c0 += blockDim.x) {
@@ -674,9 +680,8 @@ __global__ void __launch_bounds__(kListThreads, 20) loss_listed_kernel(LossArgs 
     __shared__ float scratch[kWarps];
     __shared__ NamedSums named_sums;
     const int n_words = (int)((a.n_moves + 31) / 32), n = a.n_listed;
-    unsigned *const marks = dynamic;            // the named moves, the listed ones, then the list, its logits, the named
-    unsigned *const support = dynamic + n_words;
-    int *const listed = reinterpret_cast<int *>(support + n_words);
+    unsigned *const support = dynamic;          // a bit for each listed move, the named ones taken out again; then the list, its
+    int *const listed = reinterpret_cast<int *>(support + n_words);      // logits, the named moves
     float *const at = reinterpret_cast<float *>(listed + n);
     const Named nm(reinterpret_cast<unsigned char *>(at + n), a.k, &named_sums);
     const float inv_t = 1.f / a.temperature, c = kLog2e * inv_t;
@@ -691,7 +696,6 @@ __global__ void __launch_bounds__(kListThreads, 20) loss_listed_kernel(LossArgs 
         const float weight = a.weight ? a.weight[i] : 1.f;
         T *g = grad ? grad + i * a.ld_g : nullptr;
         __syncthreads();                        // the row before is done with the shared memory
-        for (int w = threadIdx.x; w < n_words; w += kListThreads) marks[w] = 0u;
         read_list<kListThreads>(a.list + i * n, a.valid + i * n, n, a.n_moves, row, support, n_words, listed, at);
         if (g) {                                // zeros everywhere, the listed moves over them after a barrier
             constexpr int kPer = Piece<T>::kPer;
@@ -702,15 +706,13 @@ __global__ void __launch_bounds__(kListThreads, 20) loss_listed_kernel(LossArgs 
             if ((int)threadIdx.x < head) g[threadIdx.x] = from_float<T>(0.f);
             if (tail + (int)threadIdx.x < moves) g[tail + threadIdx.x] = from_float<T>(0.f);
         }
-        read_named(nm, a, i, row, first_named, [&](int m) { return ((support[m >> 5] >> (m & 31)) & 1u) != 0u; },
-                   [&](int m) { return to_float(row[m]); }, [&](int m) { return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u); });
+        auto in_support = [&](int m) { return ((support[m >> 5] >> (m & 31)) & 1u) != 0u; };
+        read_named<true>(nm, a, i, row, first_named, in_support, [&](int m) { return to_float(row[m]); },
+                         [&](int m) { return (int)((~atomicAnd(&support[m >> 5], ~(1u << (m & 31))) >> (m & 31)) & 1u); });
         const int role = (int)(threadIdx.x >> 5);
         if (role == 0) sum_named(nm, a.k, c);
         else if (role == 1) teach(nm, a, i, c, inv_t);
-        auto other = [&](int e) {               // the e-th listed move is in the support and not named
-            const int m = listed[e];
-            return m >= 0 && !((marks[m >> 5] >> (m & 31)) & 1u);
-        };
+        auto other = [&](int e) { return listed[e] >= 0 && in_support(listed[e]); };     // takes part and is not named
         float m = -kInf, sum = 0.f;
         for (int e = threadIdx.x; e < n; e += kListThreads)
             if (other(e)) m = fmaxf(m, at[e]);
@@ -808,7 +810,7 @@ __global__ void __launch_bounds__(NT, 768 / NT) loss_kernel(LossArgs a, int64_t 
             copies_done<0>();
         }
         __syncthreads();
-        read_named(nm, a, i, row, first_named, [](int) { return true; }, [&](int m) { return to_float(held[shift + m]); },
+        read_named<false>(nm, a, i, row, first_named, [](int) { return true; }, [&](int m) { return to_float(held[shift + m]); },
                    [&](int m) {
                        held[shift + m] = from_float<T>(-kInf);
                        return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u);
@@ -925,7 +927,7 @@ __global__ void __launch_bounds__(kLongThreads) loss_long_kernel(LossArgs a, int
         __syncthreads();                        // the row before is done with the shared memory
         for (int w = threadIdx.x; w < words; w += kLongThreads) marks[w] = 0u;
         __syncthreads();
-        read_named(nm, a, i, row, first_named, [](int) { return true; }, [&](int m) { return to_float(row[m]); },
+        read_named<false>(nm, a, i, row, first_named, [](int) { return true; }, [&](int m) { return to_float(row[m]); },
                    [&](int m) { return (int)((atomicOr(&marks[m >> 5], 1u << (m & 31)) >> (m & 31)) & 1u); });
         if (warp == 0) sum_named(nm, a.k, c);
         else if (warp == 1) teach(nm, a, i, c, inv_t);
@@ -1112,7 +1114,7 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
             const T *x = static_cast<const T *>(logits);
             T *g = static_cast<T *>(grad);
             if (legal) {
-                const size_t shared = (size_t)((n_moves + 31) / 32) * 8 + (size_t)n_listed * 8 + Named::bytes(k);
+                const size_t shared = (size_t)((n_moves + 31) / 32) * 4 + (size_t)n_listed * 8 + Named::bytes(k);
                 allow_shared<loss_listed_kernel<T>>(shared);
                 // a call that may have nothing to do is not worth a CTA per row
                 const unsigned grid = (unsigned)(skip_ones ? std::min<int64_t>(rows, 148 * 8) : rows);

@@ -57,3 +57,26 @@ def test_selection_repeats_bit_for_bit(rows, v, k, dtype):
         again = top_logits(x, k, 2.0)
         for a, b in zip(first[:3], again[:3]):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_lists_over_the_most_moves(dtype):
+    """1,048,576 moves with the longest lists and the most named moves: the loss over the lists is that of the listed
+    logits side by side."""
+    v, listed, k = 1 << 20, 4096, 256
+    x = torch.zeros(2, v, dtype=dtype, device=DEV)
+    moves = torch.stack([torch.randperm(v, device=DEV, generator=torch.Generator(device=DEV).manual_seed(i))[:listed].sort().values for i in range(2)])
+    moves[:, -1] = v - 1
+    x.scatter_(1, moves, (_rand(2, listed, seed=3) * 2).to(dtype))
+    legal = moves, torch.rand(2, listed, device=DEV, generator=torch.Generator(device=DEV).manual_seed(5)) < 0.9
+    side = x.gather(1, moves).masked_fill(~legal[1], -INF)
+    top, near = top_logits(x, k, 1.5, legal=legal), top_logits(side, k, 1.5)
+    assert torch.equal(top.values, near.values) and torch.equal(top.moves, moves.gather(1, near.moves))
+    leaf, leaf2 = x.clone().requires_grad_(True), side.clone().requires_grad_(True)
+    losses = distillation_loss(leaf, top, legal=legal, rest=True, reduction="none")
+    losses2 = distillation_loss(leaf2, near._replace(log_rest=top.log_rest), rest=True, reduction="none")
+    # two orders of the same float32 sums
+    torch.testing.assert_close(losses, losses2, rtol=1e-5, atol=1e-5)
+    g, g2 = torch.autograd.grad(losses.sum(), leaf)[0], torch.autograd.grad(losses2.sum(), leaf2)[0]
+    torch.testing.assert_close(g.gather(1, moves).float(), g2.float(), rtol=2.0**-7 if dtype == torch.bfloat16 else 2.0**-10, atol=1e-6)
+    assert int((g != 0).sum()) <= int(legal[1].sum())
