@@ -24,11 +24,14 @@ struct Error : std::runtime_error {
 
 void set_last_error(const std::string &msg);
 
+// A failed call is reported once: the runtime keeps its error until it is asked for, and the next launch would find it.
 #define AFB_CUDA(call)                                                                          \
     do {                                                                                        \
         cudaError_t err_ = (call);                                                              \
-        if (err_ != cudaSuccess)                                                                \
+        if (err_ != cudaSuccess) {                                                              \
+            (void)cudaGetLastError();                                                           \
             throw ::afb::Error(AFB_ECUDA, std::string(#call) + ": " + cudaGetErrorString(err_)); \
+        }                                                                                       \
     } while (0)
 
 #define AFB_CHECK(cond, msg)                                                  \
