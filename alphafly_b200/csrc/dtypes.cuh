@@ -1,10 +1,11 @@
 // Shared pieces of the 8-bit products and of distillation: element types (AFB_T_*), their conversions and dispatch, 16-byte
-// pieces of rows, launch sizes.
+// pieces of rows.
 #pragma once
 
 #include <cuda_bf16.h>
 
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace afb {
 
@@ -75,35 +76,6 @@ void with_type(int t, F &&f) {
     if (t == AFB_T_F32) f(float{});
     else if (t == AFB_T_F16) f(__half{});
     else f(__nv_bfloat16{});
-}
-
-// Lets the kernel take that much dynamic shared memory on the current device; asked for once per size that is needed.
-template <auto kKernel>
-void allow_shared(size_t bytes) {
-    static size_t allowed[64] = {0};
-    if (bytes <= 32 * 1024) return;
-    int dev = 0;
-    AFB_CUDA(cudaGetDevice(&dev));
-    if (dev < 64 && allowed[dev] >= bytes) return;
-    AFB_CUDA(cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (dev < 64) allowed[dev] = bytes;
-}
-
-// CTAs of a kernel that the current device holds at once (asked for again when the shared memory changes).
-template <auto kKernel>
-int64_t resident(int threads, size_t shared) {
-    static size_t of[64] = {0};
-    static int64_t ctas[64] = {0};
-    int dev = 0;
-    AFB_CUDA(cudaGetDevice(&dev));
-    if (dev < 64 && ctas[dev] && of[dev] == shared) return ctas[dev];
-    int per_sm = 0, sms = 0;
-    AFB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kKernel, threads, shared));
-    AFB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    AFB_CHECK(per_sm >= 1, "the kernel does not fit on this device");
-    const int64_t n = (int64_t)per_sm * sms;
-    if (dev < 64) of[dev] = shared, ctas[dev] = n;
-    return n;
 }
 
 }  // namespace afb

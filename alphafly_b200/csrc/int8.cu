@@ -603,10 +603,10 @@ struct PairLaunch {
 
 template <typename O>
 int device_pairs() {
-    static int pairs[64] = {0};
-    int dev = 0;
-    AFB_CUDA(cudaGetDevice(&dev));
-    AFB_CHECK(dev >= 0 && dev < 64, "device index out of range");
+    static std::mutex lock;
+    static int pairs[kMaxDevices] = {0};
+    const int dev = current_device();
+    const std::lock_guard<std::mutex> held(lock);
     if (!pairs[dev]) {
         AFB_CUDA(cudaFuncSetAttribute(pair_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
         int sms = 0, n = 0;

@@ -80,3 +80,25 @@ def test_lists_over_the_most_moves(dtype):
     g, g2 = torch.autograd.grad(losses.sum(), leaf)[0], torch.autograd.grad(losses2.sum(), leaf2)[0]
     torch.testing.assert_close(g.gather(1, moves).float(), g2.float(), rtol=2.0**-7 if dtype == torch.bfloat16 else 2.0**-10, atol=1e-6)
     assert int((g != 0).sum()) <= int(legal[1].sum())
+
+
+def test_calls_from_several_threads():
+    """Threads that need different amounts of a kernel's shared memory get what one thread would."""
+    from concurrent.futures import ThreadPoolExecutor
+    cases = []
+    for n, v in enumerate((30000, 70000, 300000, 700000, 1 << 20)):
+        x, moves = _rand(2, v, seed=n), torch.arange(0, v, v // 50, device=DEV).repeat(2, 1)
+        legal = moves, torch.ones_like(moves, dtype=torch.bool)
+        cases += [(x, top_logits(x, 9), None), (x, top_logits(x, 9, legal=legal), legal)]
+    torch.cuda.synchronize()
+
+    def run(i):
+        x, top, legal = cases[i % len(cases)]
+        return distillation_loss(x, top, legal=legal, rest=True, reduction="none")
+    order = [i * 7 % len(cases) for i in range(60)]
+    with ThreadPoolExecutor(6) as pool:
+        got = list(pool.map(run, order))
+    torch.cuda.synchronize()
+    ref = [run(i) for i in range(len(cases))]
+    for i, losses in zip(order, got):
+        assert torch.equal(losses, ref[i])

@@ -18,3 +18,7 @@ def _run(name, tmp_path):
 
 def test_a_failure_is_reported_once(tmp_path):
     _run("host_errors", tmp_path)
+
+
+def test_shared_memory_limits_hold_between_threads(tmp_path):
+    _run("host_shared_limit", tmp_path)
