@@ -112,11 +112,15 @@ def teacher_targets(teacher, x: torch.Tensor, k: int, temperature: float = 1.0, 
 class _Loss:
     """The arguments of one ``afb_distill_loss``, all but the student's logits."""
 
-    def __init__(self, values, moves, log_rest, temperature, legal, weight, scale):
+    def __init__(self, values, moves, log_rest, temperature, legal, weight, scale, differentiable):
         self.tensors = [t for t in (values, moves, log_rest, legal[0], legal[1], weight) if t is not None]   # for the backward
-        self.versions = [t._version for t in self.tensors]
+        self.versions = self.current_versions() if differentiable else None
         self.front = (values.shape[1], values.data_ptr(), moves.data_ptr(), _ptr(log_rest), temperature, _ptr(legal[0]),
                       _ptr(legal[1]), legal[2], _ptr(weight), scale)
+
+    def current_versions(self) -> list:
+        """What tells a change in place; tensors made in inference mode have no version."""
+        return [None if t.is_inference() else t._version for t in self.tensors]
 
     def launch(self, logits, upstream, skip_ones, rows, total, grad) -> None:
         b, n = logits.shape
@@ -150,7 +154,7 @@ class _Distillation(torch.autograd.Function):
         if torch.is_grad_enabled():
             raise RuntimeError("distillation_loss has no second derivative (create_graph)")
         logits, = ctx.saved_tensors
-        if [t._version for t in ctx.loss.tensors] != ctx.loss.versions:
+        if ctx.loss.current_versions() != ctx.loss.versions:
             raise RuntimeError("distillation_loss: a target or list was modified in place before the backward")
         grad, ctx.grad = ctx.grad, None
         skip = grad is not None
@@ -179,6 +183,7 @@ def distillation_loss(logits: torch.Tensor, top: TopLogits, legal=None, rest: bo
     log_rest = _matrix(top.log_rest, (b,), torch.float32, dev, "top.log_rest") if rest else None
     if weight is not None:
         weight = _matrix(weight.detach(), (b,), torch.float32, dev, "weight")
+    differentiable = torch.is_grad_enabled() and logits.requires_grad
     loss = _Loss(values, moves, log_rest, float(top.temperature), _legal(legal, logits), weight,
-                 1.0 / b if reduction == "mean" and b else 1.0)
-    return _Distillation.apply(logits, loss, reduction, torch.is_grad_enabled() and logits.requires_grad)
+                 1.0 / b if reduction == "mean" and b else 1.0, differentiable)
+    return _Distillation.apply(logits, loss, reduction, differentiable)

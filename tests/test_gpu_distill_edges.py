@@ -102,3 +102,33 @@ def test_calls_from_several_threads():
     ref = [run(i) for i in range(len(cases))]
     for i, losses in zip(order, got):
         assert torch.equal(losses, ref[i])
+
+
+def test_targets_made_in_inference_mode():
+    """The natural way to run a teacher; such tensors track no versions."""
+    x, t = _rand(5, 400, seed=1), _rand(5, 400, seed=2)
+    legal = torch.arange(60, device=DEV).repeat(5, 1), torch.rand(5, 60, device=DEV, generator=torch.Generator(device=DEV).manual_seed(3)) < 0.7
+    weight = torch.rand(5, device=DEV, generator=torch.Generator(device=DEV).manual_seed(4))
+    with torch.inference_mode():
+        made = top_logits(t, 6, 2.0, legal=legal)
+        lists = tuple(a.clone() for a in legal)
+        inside = distillation_loss(x, made, legal=lists, rest=True, weight=weight.clone(), reduction="none")
+        own = weight.clone()
+    plain = top_logits(t, 6, 2.0, legal=legal)
+    ref = distillation_loss(x, plain, legal=legal, rest=True, weight=weight, reduction="none")
+    assert made.values.is_inference() and torch.equal(inside, ref)
+    grads = []
+    for top, where, w in ((made, lists, own), (plain, legal, weight)):
+        leaf = x.clone().requires_grad_(True)
+        losses = distillation_loss(leaf, top, legal=where, rest=True, weight=w, reduction="none")
+        assert torch.equal(losses, ref)
+        grads.append(torch.autograd.grad(losses, leaf, torch.full_like(ref, 3.0))[0])
+    assert torch.equal(*grads)
+
+
+def test_targets_changed_before_the_backward_are_refused():
+    leaf, top = _rand(3, 50, seed=1).requires_grad_(True), top_logits(_rand(3, 50, seed=2), 4)
+    loss = distillation_loss(leaf, top)
+    top.values.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified in place"):
+        loss.backward()
