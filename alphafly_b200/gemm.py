@@ -22,7 +22,8 @@ _status: dict = {}
 def _device_status(dev: torch.device) -> torch.Tensor:
     st = _status.get(dev)
     if st is None:
-        st = _status[dev] = torch.zeros(1, dtype=torch.int32, device=dev)
+        with torch.inference_mode(False):        # written again when it is reset, in whatever mode
+            st = _status[dev] = torch.zeros(1, dtype=torch.int32, device=dev)
     return st
 
 

@@ -16,6 +16,7 @@ folded into the policy rows, float32 accuracy from split float16 operands, or 8-
 
 from __future__ import annotations
 
+import contextlib
 import dataclasses
 from collections import OrderedDict
 
@@ -68,6 +69,14 @@ class RunningNorm(nn.Module):
                 self.var.lerp_(var, m)
                 self.initialised.fill_(True)
         return ((r - self.mean) / (self.var + self.eps).sqrt()).clamp(-self.clip, self.clip)
+
+
+@contextlib.contextmanager
+def lasting():
+    """What is made in here is kept between calls and written again: ordinary tensors even where the caller is in inference
+    mode (whose tensors nothing outside it may write), without gradients."""
+    with torch.inference_mode(False), torch.no_grad():
+        yield
 
 
 class FlyChessNet(nn.Module):
@@ -133,9 +142,10 @@ class FlyChessNet(nn.Module):
         where = (w.data_ptr(), b.data_ptr(), k)
         c = getattr(self, "_enc16", None)
         if c is None or c[1] != where:
-            w16 = torch.zeros(w.shape[0], -(-k // 8) * 8, dtype=torch.float16, device=w.device)[:, :k]   # rows on 16 B
-            w16.copy_(w[:, :k])
-            c = [key, where, w16, b.half()]
+            with lasting():
+                w16 = torch.zeros(w.shape[0], -(-k // 8) * 8, dtype=torch.float16, device=w.device)[:, :k]   # rows on 16 B
+                w16.copy_(w[:, :k])
+                c = [key, where, w16, b.half()]
             self._enc16 = c
         elif c[0] != key:
             c[2].copy_(w[:, :k])
@@ -147,7 +157,8 @@ class FlyChessNet(nn.Module):
         """The input map's device status word on ``device`` (0 = ok; set when a bounded wait gave up)."""
         st = getattr(self, "_status", None)
         if st is None or st.device != device:
-            st = self._status = torch.zeros(1, dtype=torch.int32, device=device)
+            with lasting():
+                st = self._status = torch.zeros(1, dtype=torch.int32, device=device)
         return st
 
     def device_status(self, reset: bool = True) -> int:
@@ -231,8 +242,9 @@ class FlyChessNet(nn.Module):
         c = getattr(self, "_heads8", None)
         if c is not None and c[0] == key and c[1] == where:
             return c[2]
-        w, b = self._folded()
-        new = (*quantize(w), b)
+        with lasting():
+            w, b = self._folded()
+            new = (*quantize(w), b)
         if c is not None and c[1] == where:
             for old, t in zip(c[2], new):
                 old.copy_(t)
@@ -267,9 +279,10 @@ class FlyChessNet(nn.Module):
         rows, n_out = w.shape
         ldw = -(-n_out // 8) * 8
         if c is None or c[1] != where or c[2].shape != (rows, ldw):
-            hi = torch.empty(rows, ldw, dtype=torch.float16, device=w.device)
-            lo = torch.empty_like(hi)
-            bias = torch.empty(rows, dtype=torch.float32, device=w.device)
+            with lasting():
+                hi = torch.empty(rows, ldw, dtype=torch.float16, device=w.device)
+                lo = torch.empty_like(hi)
+                bias = torch.empty(rows, dtype=torch.float32, device=w.device)
         else:
             hi, lo, bias = c[2], c[3], c[4]
         bias.copy_(b)
@@ -443,6 +456,7 @@ class Evaluator:
         self._graphs[key] = entry
         return entry
 
+    @torch.inference_mode(False)                       # the graphs' inputs and the pinned buffers are written again
     @torch.no_grad()
     def submit(self, x, rows, cols):
         """Launch the evaluation and return at once; ``result`` waits for it."""
