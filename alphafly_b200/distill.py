@@ -100,12 +100,13 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=Non
 def teacher_targets(teacher, x: torch.Tensor, k: int, temperature: float = 1.0, legal=None) -> TopLogits:
     """``teacher`` (a ``FlyChessNet``) on the positions ``x`` (B, N_FEATURES), in inference: its ``top_logits``.  With
     ``teacher.infer_heads`` "int8" the readout runs in 8-bit integers."""
-    mode = teacher.training
+    modes = [(m, m.training) for m in teacher.modules()]         # a part may be frozen in a mode of its own
     teacher.eval()
     try:
         logits, _ = teacher(x)
     finally:
-        teacher.train(mode)
+        for m, training in modes:
+            m.training = training
     return top_logits(logits, k, temperature, legal)
 
 
