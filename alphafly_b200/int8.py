@@ -8,6 +8,9 @@ some of that accuracy, ``quantize`` turns a matrix into int8 with one float32 sc
 
 with exact int32 sums.  Weights are quantised once (``quantize(layer.weight)``), positions within the call.
 A row of x that holds an infinity or a NaN gives a row of NaN; the other rows do not see it.
+
+These are products of inference.  Rounding has no gradient: ``quantize`` returns none, and a backward that comes to a
+product with an input that wants one fails.
 """
 
 from __future__ import annotations
@@ -98,6 +101,24 @@ def _result(rows: int, n: int, k: int, w, w_scale, bias, out_dtype, device):
     return w, _vector(w_scale, n, device, "w_scale"), _vector(bias, n, device, "bias"), y
 
 
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, *sources):
+        return y.view_as(y)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("the 8-bit product has no gradient: detach its inputs, or run it under torch.no_grad()")
+
+
+def _without_gradient(y: torch.Tensor, *sources) -> torch.Tensor:
+    """``y``, computed from ``sources`` outside autograd: a backward that asks one of them for a gradient fails, where it
+    would otherwise pass it by."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in sources):
+        return _NoGradient.apply(y, *sources)
+    return y
+
+
 def _empty_sum(y: torch.Tensor, bias) -> torch.Tensor:
     """The product over k = 0."""
     y.zero_()
@@ -115,16 +136,17 @@ def int8_matmul(q: torch.Tensor, scale: torch.Tensor, w: torch.Tensor, w_scale: 
         raise RuntimeError("q must be a CUDA tensor")
     rows, k = q.shape
     n, dev = w.shape[0], q.device
+    sources = scale, w_scale, bias
     q = _rows16(q, dev, "q")
     scale = _vector(scale, rows, dev, "scale")
     w, w_scale, bias, y = _result(rows, n, k, w, w_scale, bias, out_dtype, dev)
     if k == 0:
-        return _empty_sum(y, bias)
+        return _without_gradient(_empty_sum(y, bias), *sources)
     with _lib.on_device(dev):
         _lib.call("afb_int8_matmul", rows, n, k, q.data_ptr(), q.stride(0), scale.data_ptr(), w.data_ptr(), w.stride(0),
                   w_scale.data_ptr(), bias.data_ptr() if bias is not None else None, y.data_ptr(), TYPES[out_dtype], y.stride(0),
                   _device_status(dev).data_ptr(), _lib.stream_of(dev))
-    return y
+    return _without_gradient(y, *sources)
 
 
 def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor | None = None, norm=None,
@@ -135,9 +157,10 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
     _check_source(x, norm)
     rows, k = x.shape
     n, dev = w.shape[0], x.device
+    sources = x, w_scale, bias
     w, w_scale, bias, y = _result(rows, n, k, w, w_scale, bias, out_dtype, dev)
     if k == 0:
-        return _empty_sum(y, bias)
+        return _without_gradient(_empty_sum(y, bias), *sources)
     x, ld, trans = _source(x)
     lib = _lib.load()
     size = lib.afb_int8_linear_workspace(rows, k)
@@ -147,4 +170,4 @@ def int8_linear(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: t
                                        w.stride(0), w_scale.data_ptr(), bias.data_ptr() if bias is not None else None,
                                        y.data_ptr(), TYPES[out_dtype], y.stride(0), ws.data_ptr() if size else None, size,
                                        _device_status(dev).data_ptr(), _lib.stream_of(dev)))
-    return y
+    return _without_gradient(y, *sources)

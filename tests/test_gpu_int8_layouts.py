@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from alphafly_b200.int8 import quantize
+from alphafly_b200.int8 import int8_linear, int8_matmul, quantize
 from alphafly_b200.model import RunningNorm
 
 pytestmark = pytest.mark.gpu
@@ -53,3 +53,24 @@ def test_quantize_across_clusters_and_spans(rows, k, dtype, with_norm, layout):
         q, scale = quantize(src, norm)
         assert np.array_equal(scale.cpu().numpy(), rs, equal_nan=True)
         assert np.array_equal(q.cpu().numpy(), rq)
+
+
+def test_a_backward_through_the_product_fails():
+    """Rather than leave what lies before the product without a gradient."""
+    x, (w, ws), bias = _rand(3, 40), quantize(_rand(6, 40, seed=1)), _rand(6, seed=2)
+    q, scale = quantize(x)
+    ref = int8_linear(x, w, ws, bias)
+    leaf = x.clone().requires_grad_(True)
+    other = torch.ones(3, 6, device=DEV, requires_grad=True)
+    for y in (int8_linear(leaf * 1.0, w, ws, bias), int8_linear(x, w, ws, bias.clone().requires_grad_(True)),
+              int8_matmul(q, scale, w, ws.clone().requires_grad_(True), bias)):
+        assert torch.equal(y, ref)
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            (y * other).sum().backward()
+    for y in (int8_linear(leaf.detach(), w, ws, bias), int8_linear(x, w, ws, bias)):
+        assert not y.requires_grad
+        (y * other).sum().backward()
+    with torch.no_grad():
+        assert not int8_linear(leaf, w, ws, bias).requires_grad
+    empty = int8_linear(torch.empty(3, 0, device=DEV, requires_grad=True), w[:, :0], ws, bias)
+    assert empty.requires_grad and torch.equal(empty, bias.expand(3, 6))
