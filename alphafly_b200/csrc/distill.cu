@@ -1045,7 +1045,9 @@ void check_rows(int64_t rows, int64_t n_moves, int type, const void *logits, int
     AFB_CHECK(n_moves <= kMaxMoves, "more than 1048576 moves");
     AFB_CHECK(known_type(type), "unknown element type");
     AFB_CHECK(k >= 1 && k <= kMaxTop, "k must be between 1 and 256");
-    AFB_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "the temperature must be positive and finite");
+    // the kernels take logits times log2(e) / T
+    AFB_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(kLog2e * (1.f / temperature)),
+              "the temperature must be positive and finite, and so its inverse");
     AFB_CHECK((list == nullptr) == (valid == nullptr), "a list of moves comes with its valid flags");
     AFB_CHECK(n_listed <= kMaxListed, "more than 4096 listed moves a position");
     AFB_CHECK(ld >= n_moves, "a leading dimension is below the row length");
@@ -1094,6 +1096,7 @@ int afb_distill_loss(int64_t rows, int64_t n_moves, int type, const void *logits
                      int skip_ones, float *row_loss, float *loss, void *grad, int64_t ld_grad, void *stream) {
     return guarded([&] {
         check_rows(rows, n_moves, type, logits, ld, k, temperature, legal, valid, n_listed);
+        AFB_CHECK(std::isfinite(temperature * temperature), "the square of the temperature must be finite");
         AFB_CHECK(upstream_step >= 0, "negative size");
         AFB_CHECK(upstream || !skip_ones, "skip_ones needs the upstream gradient");
         if (rows == 0) {

@@ -275,7 +275,8 @@ AFB_API int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, cons
  * No counterpart in the reference, which trains on visit distributions (chessfly/train.py:105-132).
  * logits: (rows, n_moves) of `type`, row stride ld, n_moves <= 1048576.  legal, valid: the moves that take
  * part, (rows, n_listed) int64 and 0 / 1 bytes, n_listed <= 4096; both NULL: all moves.  A listed move that is
- * not valid, out of range or named before in its row is ignored.  1 <= k <= 256, temperature T > 0.
+ * not valid, out of range or named before in its row is ignored.  1 <= k <= 256, temperature T > 0 (log2(e) / T,
+ * and for the loss T^2, finite in float32).
  *
  * afb_top_logits: each row's k largest logits, largest first, equal ones by the lower move, into values and
  *   moves (rows, k); NaN and -inf are never taken; places that no move fills hold -inf and -1.  log_rest
