@@ -335,9 +335,10 @@ __global__ void __launch_bounds__(kDotThreads) dot_kernel(int64_t n, int k_dim, 
     }
 }
 
-// One row that fits the shared memory of a CTA.  (Two rows are as fast on the tensor cores: 11.8 us at 2333 x 4171, where
+// One row, which fits the shared memory of a CTA.  (Two rows are as fast on the tensor cores: 11.8 us at 2333 x 4171, where
 // one row takes 7.2 here, most of it the quantisation that every CTA repeats.)
-bool one_row(int64_t rows, int64_t k) { return rows == 1 && (k + 15) / 16 * 16 <= kDotMost; }
+static_assert((kMaxK + 15) / 16 * 16 <= kDotMost, "the longest row");
+bool one_row(int64_t rows) { return rows == 1; }
 
 template <typename T, bool kFused>
 void launch_dot(int64_t n, int64_t k, const T *x, int64_t k_step, const Norm &norm, const float *q_scale, const int8_t *w, int64_t ld_w,
@@ -719,7 +720,7 @@ void quantize(int64_t rows, int64_t k, int type, const void *x, int64_t ld_x, in
 
 void matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t ld_q, const float *q_scale, const int8_t *w, int64_t ld_w,
             const float *w_scale, const float *bias, void *y, int y_type, int64_t ld_y, int *status, cudaStream_t s) {
-    if (one_row(rows, k)) {
+    if (one_row(rows)) {
         launch_dot<int8_t, false>(n, k, q, 1, Norm{}, q_scale, w, ld_w, w_scale, bias, y, y_type, s);
         return;
     }
@@ -796,7 +797,7 @@ int afb_int8_matmul(int64_t rows, int64_t n, int64_t k, const int8_t *q, int64_t
 }
 
 size_t afb_int8_linear_workspace(int64_t rows, int64_t k) {
-    if (rows <= 0 || k <= 0 || one_row(rows, k)) return 0;
+    if (rows <= 0 || k <= 0 || one_row(rows)) return 0;
     return align256((size_t)rows * round128(k)) + align256((size_t)rows * 4) + 256;
 }
 
@@ -813,7 +814,7 @@ int afb_int8_linear(int64_t rows, int64_t n, int64_t k, int x_type, const void *
         const size_t need = afb_int8_linear_workspace(rows, k);
         AFB_CHECK(need == 0 || (workspace && workspace_bytes >= need), "workspace too small (afb_int8_linear_workspace)");
         const Norm norm{mean, var, eps, clip};
-        if (one_row(rows, k)) {
+        if (one_row(rows)) {
             with_type(x_type, [&](auto t) {
                 using T = decltype(t);
                 launch_dot<T, true>(n, k, static_cast<const T *>(x), x_trans ? ld_x : 1, norm, nullptr, w, ld_w, w_scale, bias, y, y_type,
