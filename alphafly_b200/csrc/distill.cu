@@ -147,8 +147,10 @@ __device__ unsigned kth_of_groups(const unsigned *group, int k) {
     return t;
 }
 
-// Entries that are ranked without a bound: 35,840 lists of 64, k = 8: 92 us, 107 with it; of 100: 151 us, 137 with it.
-constexpr int kFew = 64;
+// Entries that are ranked without a bound.  35,840 lists of 33, 48, 64, 72, 80, 96 and 128, k = 8: 77, 87, 92, 110, 125, 141
+// and 186 us without, 105, 107, 108, 115, 122, 131 and 157 with it (k = 32 the same within 4%); fewer rows would gain up to
+// 112 entries (1,120 lists of 96: 9.9 us without, 10.7 with).
+constexpr int kFew = 72;
 
 // Selects from `n` entries, get(e, order, move).  A row with too many entries at the bound (many equal values) finds
 // the k-th key itself bit by bit.
@@ -284,9 +286,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // Candidates that one warp ranks by itself where many rows keep the SM busy (35,840 x 4168 float32, k = 128: 363 us, 406 with
-// the whole CTA; a single row of k = 64: 6.7 us and 6.0), fewer in larger CTAs (2,048 x 32000 bfloat16, k = 64: 57 and 59 us with
-// 96 and 160).
-constexpr int kRanked = 160, kManyRows = 256;
+// the whole CTA; a single row of k = 64: 6.7 us and 6.0).  Fewer in larger CTAs, of which an SM holds few.  With at most 64, 96
+// and 160: 2,048 x 32000 bfloat16 62, 58 and 58 us at k = 64, 67, 67 and 71 at k = 100, 71, 71 and 77 at k = 130; float32 82, 77 and
+// 78 at k = 64; 4,096 x 26000 float16 112, 102 and 102 at k = 64.  More rows would take more: 8,000 x 12000 float32 119, 107 and
+// 99 at k = 64, 157, 157 and 153 at k = 130.
+constexpr int kRanked = 160, kRankedLarge = 96, kManyRows = 256;
 
 // The largest of each of four subsets of a thread's moves (a maximum passes NaN over); 16-bit types two at a time.
 template <typename T>
@@ -487,7 +491,7 @@ __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restric
     auto block_sync = [] { __syncthreads(); };
     auto warp_sync = [] { __syncwarp(); };
     using std::integral_constant;
-    constexpr int kAlone = NT == kThreads ? kRanked : 96;
+    constexpr int kAlone = NT == kThreads ? kRanked : kRankedLarge;
     if (found > (gridDim.x >= kManyRows ? kAlone : 32)) {
         if (found <= NT) close((int)threadIdx.x, NT, integral_constant<int, 1>{}, in_block, block_sync);
         else if (found <= 2 * NT) close((int)threadIdx.x, NT, integral_constant<int, 2>{}, in_block, block_sync);
