@@ -47,11 +47,6 @@ def _check_logits(logits: torch.Tensor, temperature: float) -> torch.Tensor:
     return logits if logits.stride(1) == 1 and logits.stride(0) >= logits.shape[1] else logits.contiguous()
 
 
-def _row_stride(logits: torch.Tensor) -> int:
-    """From one row to the next; a single row's stride says nothing (torch leaves any number there)."""
-    return max(logits.stride(0), logits.shape[1])
-
-
 def _matrix(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device, name: str) -> torch.Tensor:
     if tuple(t.shape) != shape or t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must be {dtype} {shape} on the logits' device, got {t.dtype} {tuple(t.shape)} on {t.device}")
@@ -89,8 +84,9 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=Non
     moves, valid, listed = _legal(legal, logits)
     out = TopLogits(torch.empty(b, k, dtype=torch.float32, device=dev), torch.empty(b, k, dtype=torch.int64, device=dev),
                     torch.empty(b, dtype=torch.float32, device=dev), float(temperature))
+    ld = logits.stride(0) if b > 1 else n        # a single row's stride says nothing: torch leaves any number there
     with _lib.on_device(dev):
-        _lib.call("afb_top_logits", b, n, TYPES[logits.dtype], logits.data_ptr(), _row_stride(logits), k, float(temperature),
+        _lib.call("afb_top_logits", b, n, TYPES[logits.dtype], logits.data_ptr(), ld, k, float(temperature),
                   _ptr(moves), _ptr(valid), listed, out.values.data_ptr(), out.moves.data_ptr(), out.log_rest.data_ptr(),
                   _lib.stream_of(dev))
     return out
@@ -126,8 +122,9 @@ class _Loss:
     def launch(self, logits, upstream, skip_ones, rows, total, grad) -> None:
         b, n = logits.shape
         dev = logits.device
+        ld = logits.stride(0) if b > 1 else n    # as in top_logits
         with _lib.on_device(dev):
-            _lib.call("afb_distill_loss", b, n, TYPES[logits.dtype], logits.data_ptr(), _row_stride(logits), *self.front,
+            _lib.call("afb_distill_loss", b, n, TYPES[logits.dtype], logits.data_ptr(), ld, *self.front,
                       _ptr(upstream), upstream.stride(0) if upstream is not None and upstream.dim() else 0, skip_ones, _ptr(rows),
                       _ptr(total), _ptr(grad), n, _lib.stream_of(dev))
 

@@ -111,11 +111,11 @@ class _NoGradient(torch.autograd.Function):
         raise RuntimeError("the 8-bit product has no gradient: detach its inputs, or run it under torch.no_grad()")
 
 
-def _without_gradient(y: torch.Tensor, *sources) -> torch.Tensor:
-    """``y``, computed from ``sources`` outside autograd: a backward that asks one of them for a gradient fails, where it
+def _without_gradient(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor | None) -> torch.Tensor:
+    """``y``, computed from the others outside autograd: a backward that asks one of them for a gradient fails, where it
     would otherwise pass it by."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in sources):
-        return _NoGradient.apply(y, *sources)
+    if torch.is_grad_enabled() and (a.requires_grad or b.requires_grad or (c is not None and c.requires_grad)):
+        return _NoGradient.apply(y, a, b, c)
     return y
 
 
