@@ -319,8 +319,8 @@ struct FourMax<float> {
 
 // All moves of a row: one CTA per row, of NT threads, P pieces a thread in registers (P = 0: any length, the row is read
 // twice, the second time from cache).  One pass takes the groups' maxima, one collects the moves at or above the bound
-// and sums the exponentials of the others relative to it; one warp ranks the candidates.  35,840 x 4168 float32: 113 us
-// for k = 1 (5.3 TB/s), 159 for 32, 363 for 128; 2,048 x 32000 bfloat16, k = 64: 57 us.  Bound by what a row costs beside
+// and sums the exponentials of the others relative to it; one warp ranks the candidates.  35,840 x 4168 float32: 112 us
+// for k = 1 (5.3 TB/s), 160 for 32, 361 for 128; 2,048 x 32000 bfloat16, k = 64: 58 us.  Bound by what a row costs beside
 // its elements: the search for the bound and the ranking are one warp's, while the other CTAs of the SM load.
 template <typename T, int NT, int P>
 __global__ void __launch_bounds__(NT) top_kernel(int n_moves, const T *__restrict__ logits, int64_t ld, int k, float inv_t,
@@ -771,8 +771,8 @@ __device__ __forceinline__ void fetch_row(T *held, const T *row, int n) {
 // (into a second buffer) while it works on one, so that only shared memory is waited for.  The named moves are taken out
 // of the row (-inf), so that its sum is the rest's.  The terms are relative to the teacher's best move: no maximum is
 // taken, one barrier joins the sums.  Sums outside kSmall .. kLarge (logits 69 T from that move's, no such move, NaN,
-// values whose product with 1 / T overflows) are taken again, after subtracting the largest.  35,840 x 4168 float32: 203
-// us with the gradient (5.9 TB/s of reads and writes), 144 without; 4,096 x 32000 bfloat16 with it 113 us (4.6 TB/s), where
+// values whose product with 1 / T overflows) are taken again, after subtracting the largest.  35,840 x 4168 float32: 205
+// us with the gradient (5.8 TB/s of reads and writes), 145 without; 4,096 x 32000 bfloat16 with it 113 us (4.6 TB/s), where
 // the exponentials, each taken twice, fill half of their pipe's time.
 constexpr float kSmall = 1e-30f, kLarge = 1e30f;
 

@@ -73,8 +73,8 @@ def _ptr(t: torch.Tensor | None):
 
 
 def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0, legal=None) -> TopLogits:
-    """The k (at most 256) largest of each row of ``logits`` (B, moves), equal ones by the lower move; -inf and NaN
-    are never taken.  ``legal``: (moves (B, K) int64, valid (B, K) bool), as a ``train.Batch`` holds them, restricts
+    """The k (at most 256) largest of each row of ``logits`` (B, moves), equal ones by the lower move, without gradients;
+    -inf and NaN are never taken.  ``legal``: (moves (B, K) int64, valid (B, K) bool), as a ``train.Batch`` holds them, restricts
     a row to its listed moves; a row without any comes back as -inf / -1."""
     logits = _check_logits(logits, temperature)
     if not 1 <= k <= 256:
@@ -168,7 +168,7 @@ def distillation_loss(logits: torch.Tensor, top: TopLogits, legal=None, rest: bo
     gradient by ``logits``: float32, the mean over the B positions, their sum, or (B,) with ``reduction`` "none".
     ``legal``: the lists that restrict the student's softmax (as for ``top_logits``); a named move outside them is
     left out.  ``rest``: the moves the teacher does not name count as one outcome.  ``weight`` (B,) float32 scales
-    the positions' losses.  A position without a named move contributes zero."""
+    the positions' losses (no gradient goes to it or to ``top``).  A position without a named move contributes zero."""
     logits = _check_logits(logits, top.temperature)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"unknown reduction {reduction!r}")

@@ -258,7 +258,7 @@ AFB_API int afb_gemm_f32(int64_t p, int64_t q, int64_t k, float alpha, const flo
  *   bias (n) float32 or NULL.  y[i * ld_y + j] of y_type, rounded once.  status: optional device int, OR-ed
  *   with a non-zero code if one of the kernel's bounded waits gave up (never expected).
  * afb_int8_linear: both, x quantised into the workspace (afb_int8_linear_workspace bytes, 0 for one
- *   row of at most 131072 elements; one call at a time per workspace).  All asynchronous on `stream`. */
+ *   row; one call at a time per workspace).  All asynchronous on `stream`. */
 AFB_API int afb_quantize_rows(int64_t rows, int64_t k, int x_type, const void *x, int64_t ld_x, int x_trans,
                               const float *mean, const float *var, float eps, float clip, int8_t *q, int64_t ld_q,
                               float *scale, void *stream);
