@@ -605,7 +605,8 @@ __device__ __forceinline__ void teach(const Named &nm, const LossArgs &a, int64_
         if (nm.move[e] >= 0) sz += exp2_fast((nm.z[e] - mz) * c);
     sz = warp_reduce(sz, Sum());
     const float log_sz = logf(sz), log_rest = a.log_rest ? a.log_rest[i] : -kInf;
-    const float odds = mz * inv_t - log_rest + log_sz;                   // inf without a rest
+    // inf without a rest, also where mz / T leaves the range (a mask of the type's lowest value, T < 1)
+    const float odds = log_rest == -kInf ? kInf : mz * inv_t - log_rest + log_sz;
     const float log_p_rest = -softplus(odds), log_p_named = -softplus(-odds);
     for (int e = lane; e < a.k; e += 32)
         if (nm.move[e] >= 0) {

@@ -241,3 +241,22 @@ def test_loss_over_lists_of_many_rows(rows, v, listed, k, dtype, rest):
     top.moves[1::9, 0] = torch.randint(0, v, (len(top.moves[1::9]),), device=DEV, generator=_gen(3))
     up = torch.where(torch.rand(rows, device=DEV, generator=_gen(4)) < 0.5, 1.0, 0.25)
     _check_loss(s, top, (moves, valid), rest, torch.rand(rows, device=DEV, generator=_gen(5)), up)
+
+
+@pytest.mark.parametrize("t", [0.5, 1.0, 2.0])
+@pytest.mark.parametrize("v,listed", [(600, 0), (600, 60), (32000, 0)])
+@pytest.mark.parametrize("rest", [False, True])
+def test_teachers_masked_by_the_lowest_value(t, v, listed, rest):
+    """A teacher whose illegal moves hold the type's lowest value, in one row all of them: over a temperature below 1 they leave
+    float32's range."""
+    teacher, s = _rand(5, v, seed=1) * 2, _rand(5, v, seed=2) * 1.5
+    lowest = torch.finfo(F32).min
+    teacher[0] = lowest
+    teacher[1, 30:] = lowest
+    teacher[2, 3:] = lowest
+    legal = None
+    if listed:
+        legal = torch.arange(listed, device=DEV).repeat(5, 1), torch.ones(5, listed, dtype=torch.bool, device=DEV)
+    top = top_logits(teacher, 8, t, legal)
+    assert (top.moves >= 0).all() and not top.log_rest.isnan().any()
+    _check_loss(s, top, legal, rest)
